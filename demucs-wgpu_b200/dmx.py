@@ -16,6 +16,8 @@ LIB_PATH = os.path.join(HERE, "libdmx_cuda.so")
 SEGMENT = 343980
 
 FP32, TF32, BF16, TF32X3 = 0, 1, 2, 3
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # dmx_type, the operators' element types
+ACT_NONE, ACT_GELU = 0, 1                # dmx_activation
 
 # The symbols include/dmx.h declares, in order.
 EXPORTS = (
@@ -29,6 +31,9 @@ EXPORTS = (
     "dmx_set_stage_timing", "dmx_stage_times", "dmx_kernel_launches", "dmx_stream",
     "dmx_synchronize", "dmx_read_tensor", "dmx_shift_offsets", "dmx_ipc_export", "dmx_ipc_open",
     "dmx_ipc_close", "dmx_rows_copy", "dmx_rows_add", "dmx_separate_track_windowed",
+    "dmx_ops_create", "dmx_ops_destroy", "dmx_ops_check", "dmx_layer_norm",
+    "dmx_layer_norm_backward_workspace", "dmx_layer_norm_backward", "dmx_quantize_rows",
+    "dmx_layer_norm_quantize", "dmx_quantized_linear",
 )
 
 _f32p = ctypes.POINTER(ctypes.c_float)
@@ -157,6 +162,22 @@ def lib():
         L.dmx_stage_times.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_char_p), _f32p,
                                       ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_double),
                                       ctypes.POINTER(ctypes.c_double), ctypes.c_int]
+        vp, i64, ci = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+        L.dmx_ops_create.argtypes = [ci, ctypes.POINTER(vp)]
+        L.dmx_ops_destroy.argtypes = [vp]
+        L.dmx_ops_destroy.restype = None
+        L.dmx_ops_check.argtypes = [vp, vp]
+        L.dmx_layer_norm.argtypes = [vp, vp, ci, i64, vp, vp, ci, i64, i64, ctypes.c_float, vp, ci,
+                                     i64, vp, vp, vp]
+        L.dmx_layer_norm_backward_workspace.argtypes = [i64, i64]
+        L.dmx_layer_norm_backward_workspace.restype = ctypes.c_size_t
+        L.dmx_layer_norm_backward.argtypes = [vp, vp, ci, i64, vp, ci, i64, vp, ci, vp, vp, i64,
+                                              i64, vp, i64, vp, vp, vp, ctypes.c_size_t, vp]
+        L.dmx_quantize_rows.argtypes = [vp, vp, ci, i64, vp, i64, i64, vp, i64, vp, vp]
+        L.dmx_layer_norm_quantize.argtypes = [vp, vp, ci, i64, vp, vp, ci, i64, i64,
+                                              ctypes.c_float, vp, i64, vp, vp, vp, vp]
+        L.dmx_quantized_linear.argtypes = [vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, ci, vp,
+                                           i64, vp, ci, i64, vp]
         L.dmx_kernel_launches.restype = ctypes.c_int64
         L.dmx_kernel_launches.argtypes = [ctypes.c_void_p]
         _lib = L
@@ -471,6 +492,90 @@ class Bag:
                                                    ctypes.c_void_p(lr_ptr), n, ctypes.byref(opts),
                                                    ctypes.c_void_p(stems_ptr), PROGRESS_FN(0),
                                                    None))
+
+
+class Ops:
+    """The operators on device buffers (dmx_ops_*): layer norm, its backward
+    pass, and linear layers on 8-bit integers. Buffers are device pointers
+    (integers; 0 = not given) of ``device``, row-major with pitches in elements
+    (0 = the row length); types are TYPE_F32 / TYPE_F16 / TYPE_BF16; ``stream``
+    is a cudaStream_t as an integer, 0 the legacy default stream. The calls
+    are enqueued and do not wait; include/dmx.h has their formulas."""
+
+    def __init__(self, device: int = 0):
+        self._h = None
+        L = lib()
+        h = ctypes.c_void_p()
+        _check(L.dmx_ops_create(device, ctypes.byref(h)))
+        self._L, self._h, self.device = L, h, device
+
+    def close(self):
+        if self._h:
+            self._L.dmx_ops_destroy(self._h)
+            self._h = None
+
+    __del__ = close
+
+    def check(self, stream: int = 0):
+        """Waits for ``stream``; raises DmxError code 4 if a wait in a kernel gave up."""
+        _check(self._L.dmx_ops_check(self._h, stream))
+
+    def layer_norm(self, x: int, x_type: int, rows: int, cols: int, y: int, y_type: int,
+                   weight: int = 0, bias: int = 0, param_type: int = TYPE_F32, eps: float = 1e-5,
+                   x_ld: int = 0, y_ld: int = 0, mean: int = 0, rstd: int = 0, stream: int = 0):
+        """y = layer norm of x's rows; ``mean`` and ``rstd`` are kept for the backward pass."""
+        rc = self._L.dmx_layer_norm(self._h, x, x_type, x_ld or cols, weight, bias, param_type, rows,
+                                    cols, eps, y, y_type, y_ld or cols, mean, rstd, stream)
+        if rc:
+            _check(rc)
+
+    def layer_norm_backward_workspace(self, rows: int, cols: int) -> int:
+        """Bytes of the workspace that layer_norm_backward needs."""
+        return self._L.dmx_layer_norm_backward_workspace(rows, cols)
+
+    def layer_norm_backward(self, dy: int, dy_type: int, x: int, x_type: int, mean: int, rstd: int,
+                            rows: int, cols: int, workspace: int = 0, workspace_bytes: int = 0,
+                            weight: int = 0, param_type: int = TYPE_F32, dx: int = 0,
+                            dweight: int = 0, dbias: int = 0, dy_ld: int = 0, x_ld: int = 0,
+                            dx_ld: int = 0, stream: int = 0):
+        """dx (x's type), dweight and dbias (float32) of the layer norm; those that are 0 are left out."""
+        rc = self._L.dmx_layer_norm_backward(
+            self._h, dy, dy_type, dy_ld or cols, x, x_type, x_ld or cols, weight, param_type, mean,
+            rstd, rows, cols, dx, dx_ld or cols, dweight, dbias, workspace, workspace_bytes, stream)
+        if rc:
+            _check(rc)
+
+    def quantize_rows(self, x: int, x_type: int, rows: int, cols: int, q: int, scale: int,
+                      col_scale: int = 0, x_ld: int = 0, q_ld: int = 0, stream: int = 0):
+        """int8 q and one float32 scale per row of x (times ``col_scale``): x ~ q scale."""
+        rc = self._L.dmx_quantize_rows(self._h, x, x_type, x_ld or cols, col_scale, rows, cols, q,
+                                       q_ld or cols, scale, stream)
+        if rc:
+            _check(rc)
+
+    def layer_norm_quantize(self, x: int, x_type: int, rows: int, cols: int, q: int, scale: int,
+                            weight: int = 0, bias: int = 0, param_type: int = TYPE_F32,
+                            eps: float = 1e-5, x_ld: int = 0, q_ld: int = 0, mean: int = 0,
+                            rstd: int = 0, stream: int = 0):
+        """layer_norm and quantize_rows in one pass."""
+        rc = self._L.dmx_layer_norm_quantize(self._h, x, x_type, x_ld or cols, weight, bias,
+                                             param_type, rows, cols, eps, q, q_ld or cols, scale,
+                                             mean, rstd, stream)
+        if rc:
+            _check(rc)
+
+    def quantized_linear(self, x: int, w: int, out: int, out_type: int, rows: int,
+                         out_features: int, in_features: int, x_scale: int = 0, w_scale: int = 0,
+                         bias: int = 0, activation: int = ACT_NONE, residual: int = 0, x_ld: int = 0,
+                         w_ld: int = 0, residual_ld: int = 0, out_ld: int = 0, stream: int = 0):
+        """out = act(x w^T x_scale w_scale + bias) + residual on int8 x and w; their
+        pointers and pitches (0 = in_features) are multiples of 16 bytes."""
+        rc = self._L.dmx_quantized_linear(
+            self._h, x, x_ld or in_features, x_scale, w, w_ld or in_features, w_scale, bias, rows,
+            out_features, in_features, activation, residual, residual_ld or out_features, out,
+            out_type, out_ld or out_features, stream)
+        if rc:
+            _check(rc)
 
 
 def separate_track_multi(handles, left, right, shifts=1, overlap=0.25, batch=0, out=None,

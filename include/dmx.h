@@ -414,6 +414,101 @@ void* dmx_stream(dmx_handle* h);
 /* Waits (bounded) until the handle's stream has drained. */
 dmx_status dmx_synchronize(dmx_handle* h);
 
+/* ---------------------------------------------------------------------------
+ * Operators on caller's device buffers: the layer norm with its backward pass,
+ * and linear layers on 8-bit integers. They serve programs that build or tune
+ * transformer layers around the separator (a linear run at 8 bits, the norms
+ * in front of it trained afterwards); the reference has no 8-bit path and no
+ * gradients, so they replace nothing there.
+ *
+ * Conventions. Operands are row-major with a pitch (`*_ld`, elements between
+ * rows) of at least the row length; rows are tokens. Types are dmx_type, and
+ * arithmetic is in 32 bits: a 16-bit result is rounded once, when stored.
+ * Calls are enqueued on `stream` (a cudaStream_t of the context's device, NULL
+ * = legacy default stream), do not wait, allocate nothing and may be captured
+ * into a CUDA graph. The caller keeps every buffer alive until the stream has
+ * passed the call, and orders work of other streams on it. Outputs must not
+ * overlap inputs except where a comment says "in place". `rows` 0 is accepted:
+ * it touches no row. Results do not change from call to call. */
+typedef enum { DMX_TYPE_F32 = 0, DMX_TYPE_F16 = 1, DMX_TYPE_BF16 = 2 } dmx_type;
+typedef enum { DMX_ACT_NONE = 0, DMX_ACT_GELU = 1 } dmx_activation;
+
+/* A context of one device: the flag that dmx_quantized_linear's bounded waits
+ * raise. It may be used on any streams of the device, by one host thread at a
+ * time. dmx_ops_destroy waits for the device's work in flight. */
+typedef struct dmx_ops dmx_ops;
+dmx_status dmx_ops_create(int device, dmx_ops** out);
+void dmx_ops_destroy(dmx_ops* ops);
+/* Waits (bounded) until `stream` has drained; DMX_ERR_TIMEOUT if a wait inside
+ * a kernel of this context gave up since the last check (the flag is cleared). */
+dmx_status dmx_ops_check(dmx_ops* ops, void* stream);
+
+/* Layer norm of every row: y = (x - mean) rstd weight + bias with
+ * mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps).
+ * `weight` and `bias` (cols values of param_type) may be NULL (1 and 0);
+ * `mean` and `rstd` (rows floats each, for the backward pass) may be NULL.
+ * In place: y may be x, with x's type and pitch. */
+dmx_status dmx_layer_norm(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
+                          const void* weight, const void* bias, int param_type, int64_t rows,
+                          int64_t cols, float eps, void* y, int y_type, int64_t y_ld, float* mean,
+                          float* rstd, void* stream);
+
+/* Its backward pass, from the gradient dy of y and the forward's x, mean and
+ * rstd. With h = (x - mean) rstd and g = dy weight:
+ *   dx      = rstd (g - sum g / cols - h sum(g h) / cols)   (x_type)
+ *   dweight = sum over rows of dy h,  dbias = sum over rows of dy   (floats)
+ * Any of dx, dweight, dbias may be NULL. dweight and dbias are written, not
+ * added to (rows 0: zeros). They are summed in a fixed order through
+ * `workspace`, at least dmx_layer_norm_backward_workspace(rows, cols) bytes on
+ * a 16-byte boundary, which the call overwrites and may be reused once the
+ * stream has passed it; it may be NULL when neither is wanted. In place: dx
+ * may be dy or x, with the same type and pitch. */
+size_t dmx_layer_norm_backward_workspace(int64_t rows, int64_t cols);
+dmx_status dmx_layer_norm_backward(dmx_ops* ops, const void* dy, int dy_type, int64_t dy_ld,
+                                   const void* x, int x_type, int64_t x_ld, const void* weight,
+                                   int param_type, const float* mean, const float* rstd,
+                                   int64_t rows, int64_t cols, void* dx, int64_t dx_ld,
+                                   float* dweight, float* dbias, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* Symmetric 8-bit quantisation with one scale per row. With v = x col_scale
+ * (cols floats; NULL = 1), every step rounded to f32:
+ *   scale = max |v| / 127,  q = v / scale to the nearest integer, ties to even
+ * An all-zero row has scale 0 and q = 0. A row with a NaN has scale NaN, one
+ * with an infinity scale infinity, both q = 0, so that a product with them is
+ * NaN. Rows of tokens or of a weight matrix (output channels) alike. */
+dmx_status dmx_quantize_rows(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
+                             const float* col_scale, int64_t rows, int64_t cols, int8_t* q,
+                             int64_t q_ld, float* scale, void* stream);
+
+/* dmx_layer_norm followed by dmx_quantize_rows, in one pass: y is quantised
+ * before it would be rounded to a stored type. */
+dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
+                                   const void* weight, const void* bias, int param_type,
+                                   int64_t rows, int64_t cols, float eps, int8_t* q, int64_t q_ld,
+                                   float* scale, float* mean, float* rstd, void* stream);
+
+/* Linear layer on 8-bit integers, one scale per row (token) of x and one per
+ * row (output channel) of w (out_features x in_features):
+ *   out = act(acc x_scale[row] w_scale[channel] + bias[channel]) + residual
+ * where acc is the exact integer sum over in_features (at most 131071, so that
+ * it fits 32 bits for all int8 values). x_scale, w_scale, bias (floats) and
+ * residual (out's type) may be NULL (1, 1, 0, 0). x and w start on 16-byte
+ * boundaries and their pitches are multiples of 16; the bytes between a row's
+ * end and its pitch are not used. DMX_ACT_GELU is 0.5 z (1 + erf(z / sqrt 2)).
+ * In place: residual may be out, with the same pitch.
+ *
+ * The gradient of such a layer with regard to its real input (weights kept,
+ * rounding passed straight through) is the same operator: quantise dy with
+ * col_scale = w_scale, and multiply by the transposed integers with w_scale
+ * NULL. */
+dmx_status dmx_quantized_linear(dmx_ops* ops, const int8_t* x, int64_t x_ld, const float* x_scale,
+                                const int8_t* w, int64_t w_ld, const float* w_scale,
+                                const float* bias, int64_t rows, int64_t out_features,
+                                int64_t in_features, int activation, const void* residual,
+                                int64_t residual_ld, void* out, int out_type, int64_t out_ld,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
