@@ -77,15 +77,46 @@ void check_in_place(const char* what, const void* x, int x_type, int64_t x_ld, c
     refuse(what, "in place needs one type and one pitch");
 }
 
-void check_norm(const char* what, const RowArgs& a) {
-  if (a.weight || a.bias) {
-    const size_t b = type_bytes(what, "param_type", a.param_type);
-    check_vector(what, "weight", a.weight, b, false);
-    check_vector(what, "bias", a.bias, b, false);
+void check_call(const char* what, const dmx_ops* ops, const void* args) {
+  if (!ops) refuse(what, "ops is null");
+  if (!args) refuse(what, "args is null");
+}
+
+// The fields that dmx_layer_norm and dmx_layer_norm_quantize share.
+template <typename Args>
+void set_norm(const char* what, const Args* g, RowArgs* a) {
+  if (g->weight || g->bias) {
+    const size_t b = type_bytes(what, "param_type", g->param_type);
+    check_vector(what, "weight", g->weight, b, false);
+    check_vector(what, "bias", g->bias, b, false);
   }
-  if (!(a.eps >= 0.f) || std::isinf(a.eps)) refuse(what, "eps must be finite and not negative");
-  check_vector(what, "mean", a.mean, 4, false);
-  check_vector(what, "rstd", a.rstd, 4, false);
+  if (!(g->eps >= 0.f) || std::isinf(g->eps)) refuse(what, "eps must be finite and not negative");
+  check_vector(what, "mean", g->mean, 4, false);
+  check_vector(what, "rstd", g->rstd, 4, false);
+  a->norm = true;
+  a->weight = g->weight;
+  a->bias = g->bias;
+  a->param_type = g->param_type;
+  a->eps = g->eps;
+  a->mean = g->mean;
+  a->rstd = g->rstd;
+  a->rows = g->rows;
+  a->cols = (int)g->cols;
+}
+
+// The fields that dmx_quantize_rows and dmx_layer_norm_quantize share.
+template <typename Args>
+void set_quantized(const char* what, const Args* g, size_t x_bytes, RowArgs* a) {
+  a->x = g->x;
+  a->x_type = g->x_type;
+  a->x_ld = g->x_ld ? g->x_ld : g->cols;
+  a->q = g->q;
+  a->q_ld = g->q_ld ? g->q_ld : g->cols;
+  a->scale = g->scale;
+  check_rows(what, "x", a->x, x_bytes, a->x_ld, g->cols);
+  check_rows(what, "q", a->q, 1, a->q_ld, g->cols);
+  check_vector(what, "scale", g->scale, 4, true);
+  if (static_cast<const void*>(g->q) == g->x) refuse(what, "q must not be x");
 }
 
 template <typename F>
@@ -160,36 +191,25 @@ dmx_status dmx_ops_check(dmx_ops* ops, void* stream) {
   });
 }
 
-dmx_status dmx_layer_norm(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
-                          const void* weight, const void* bias, int param_type, int64_t rows,
-                          int64_t cols, float eps, void* y, int y_type, int64_t y_ld, float* mean,
-                          float* rstd, void* stream) {
+dmx_status dmx_layer_norm(dmx_ops* ops, const dmx_layer_norm_args* g, void* stream) {
   return guarded([&] {
     const char* what = "dmx_layer_norm";
-    if (!ops) refuse(what, "ops is null");
-    check_shape(what, rows, cols);
+    check_call(what, ops, g);
+    check_shape(what, g->rows, g->cols);
     RowArgs a;
-    const size_t xb = type_bytes(what, "x_type", x_type), yb = type_bytes(what, "y_type", y_type);
-    a.norm = true;
-    a.weight = weight;
-    a.bias = bias;
-    a.param_type = param_type;
-    a.eps = eps;
-    a.mean = mean;
-    a.rstd = rstd;
-    check_norm(what, a);
-    if (rows == 0) return;
-    check_rows(what, "x", x, xb, x_ld, cols);
-    check_rows(what, "y", y, yb, y_ld, cols);
-    check_in_place(what, x, x_type, x_ld, y, y_type, y_ld);
-    a.x = x;
-    a.x_type = x_type;
-    a.x_ld = x_ld;
-    a.rows = rows;
-    a.cols = (int)cols;
-    a.y = y;
-    a.y_type = y_type;
-    a.y_ld = y_ld;
+    const size_t xb = type_bytes(what, "x_type", g->x_type);
+    const size_t yb = type_bytes(what, "y_type", g->y_type);
+    set_norm(what, g, &a);
+    if (g->rows == 0) return;
+    a.x = g->x;
+    a.x_type = g->x_type;
+    a.x_ld = g->x_ld ? g->x_ld : g->cols;
+    a.y = g->y;
+    a.y_type = g->y_type;
+    a.y_ld = g->y_ld ? g->y_ld : g->cols;
+    check_rows(what, "x", a.x, xb, a.x_ld, g->cols);
+    check_rows(what, "y", a.y, yb, a.y_ld, g->cols);
+    check_in_place(what, a.x, a.x_type, a.x_ld, a.y, a.y_type, a.y_ld);
     OnDevice on(ops->device);
     launch_rows(a, static_cast<cudaStream_t>(stream));
     CK(cudaGetLastError());
@@ -201,175 +221,137 @@ size_t dmx_layer_norm_backward_workspace(int64_t rows, int64_t cols) {
   return norm_grad_workspace(rows, cols);
 }
 
-dmx_status dmx_layer_norm_backward(dmx_ops* ops, const void* dy, int dy_type, int64_t dy_ld,
-                                   const void* x, int x_type, int64_t x_ld, const void* weight,
-                                   int param_type, const float* mean, const float* rstd,
-                                   int64_t rows, int64_t cols, void* dx, int64_t dx_ld,
-                                   float* dweight, float* dbias, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+dmx_status dmx_layer_norm_backward(dmx_ops* ops, const dmx_layer_norm_backward_args* g,
+                                   void* stream) {
   return guarded([&] {
     const char* what = "dmx_layer_norm_backward";
-    if (!ops) refuse(what, "ops is null");
-    check_shape(what, rows, cols);
-    const size_t dyb = type_bytes(what, "dy_type", dy_type), xb = type_bytes(what, "x_type", x_type);
-    if (weight) check_vector(what, "weight", weight, type_bytes(what, "param_type", param_type), false);
-    check_vector(what, "dweight", dweight, 4, false);
-    check_vector(what, "dbias", dbias, 4, false);
+    check_call(what, ops, g);
+    check_shape(what, g->rows, g->cols);
+    const size_t dyb = type_bytes(what, "dy_type", g->dy_type);
+    const size_t xb = type_bytes(what, "x_type", g->x_type);
+    if (g->weight)
+      check_vector(what, "weight", g->weight, type_bytes(what, "param_type", g->param_type), false);
+    check_vector(what, "dweight", g->dweight, 4, false);
+    check_vector(what, "dbias", g->dbias, 4, false);
     NormGradArgs a;
-    if (rows > 0) {
-      check_rows(what, "dy", dy, dyb, dy_ld, cols);
-      check_rows(what, "x", x, xb, x_ld, cols);
-      check_vector(what, "mean", mean, 4, true);
-      check_vector(what, "rstd", rstd, 4, true);
-      if (dx) {
-        check_rows(what, "dx", dx, xb, dx_ld, cols);
-        check_in_place(what, dy, dy_type, dy_ld, dx, x_type, dx_ld);
-        check_in_place(what, x, x_type, x_ld, dx, x_type, dx_ld);
+    a.dy = g->dy;
+    a.dy_type = g->dy_type;
+    a.dy_ld = g->dy_ld ? g->dy_ld : g->cols;
+    a.x = g->x;
+    a.x_type = g->x_type;
+    a.x_ld = g->x_ld ? g->x_ld : g->cols;
+    a.weight = g->weight;
+    a.param_type = g->param_type;
+    a.mean = g->mean;
+    a.rstd = g->rstd;
+    a.rows = g->rows;
+    a.cols = (int)g->cols;
+    a.dx = g->dx;
+    a.dx_ld = g->dx_ld ? g->dx_ld : g->cols;
+    a.dweight = g->dweight;
+    a.dbias = g->dbias;
+    a.partials = static_cast<float*>(g->workspace);
+    if (g->rows > 0) {
+      check_rows(what, "dy", a.dy, dyb, a.dy_ld, g->cols);
+      check_rows(what, "x", a.x, xb, a.x_ld, g->cols);
+      check_vector(what, "mean", a.mean, 4, true);
+      check_vector(what, "rstd", a.rstd, 4, true);
+      if (a.dx) {
+        check_rows(what, "dx", a.dx, xb, a.dx_ld, g->cols);
+        check_in_place(what, a.dy, a.dy_type, a.dy_ld, a.dx, a.x_type, a.dx_ld);
+        check_in_place(what, a.x, a.x_type, a.x_ld, a.dx, a.x_type, a.dx_ld);
       }
-      if (dweight || dbias) {
-        if (workspace_bytes < norm_grad_workspace(rows, cols))
+      if (a.dweight || a.dbias) {
+        if (g->workspace_bytes < norm_grad_workspace(g->rows, g->cols))
           refuse(what, "the workspace is smaller than dmx_layer_norm_backward_workspace says");
-        check_vector(what, "workspace", workspace, 16, true);
+        check_vector(what, "workspace", g->workspace, 16, true);
       }
     }
-    a.dy = dy;
-    a.dy_type = dy_type;
-    a.dy_ld = dy_ld;
-    a.x = x;
-    a.x_type = x_type;
-    a.x_ld = x_ld;
-    a.weight = weight;
-    a.param_type = param_type;
-    a.mean = mean;
-    a.rstd = rstd;
-    a.rows = rows;
-    a.cols = (int)cols;
-    a.dx = dx;
-    a.dx_ld = dx_ld;
-    a.dweight = dweight;
-    a.dbias = dbias;
-    a.partials = static_cast<float*>(workspace);
     OnDevice on(ops->device);
     launch_norm_grad(a, static_cast<cudaStream_t>(stream));
     CK(cudaGetLastError());
   });
 }
 
-dmx_status dmx_quantize_rows(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
-                             const float* col_scale, int64_t rows, int64_t cols, int8_t* q,
-                             int64_t q_ld, float* scale, void* stream) {
+dmx_status dmx_quantize_rows(dmx_ops* ops, const dmx_quantize_rows_args* g, void* stream) {
   return guarded([&] {
     const char* what = "dmx_quantize_rows";
-    if (!ops) refuse(what, "ops is null");
-    check_shape(what, rows, cols);
+    check_call(what, ops, g);
+    check_shape(what, g->rows, g->cols);
+    const size_t xb = type_bytes(what, "x_type", g->x_type);
+    check_vector(what, "col_scale", g->col_scale, 4, false);
+    if (g->rows == 0) return;
     RowArgs a;
-    const size_t xb = type_bytes(what, "x_type", x_type);
-    check_vector(what, "col_scale", col_scale, 4, false);
-    if (rows == 0) return;
-    check_rows(what, "x", x, xb, x_ld, cols);
-    check_rows(what, "q", q, 1, q_ld, cols);
-    check_vector(what, "scale", scale, 4, true);
-    if (static_cast<const void*>(q) == x) refuse(what, "q must not be x");
-    a.x = x;
-    a.x_type = x_type;
-    a.x_ld = x_ld;
-    a.col_scale = col_scale;
-    a.rows = rows;
-    a.cols = (int)cols;
-    a.q = q;
-    a.q_ld = q_ld;
-    a.scale = scale;
+    a.rows = g->rows;
+    a.cols = (int)g->cols;
+    a.col_scale = g->col_scale;
+    set_quantized(what, g, xb, &a);
     OnDevice on(ops->device);
     launch_rows(a, static_cast<cudaStream_t>(stream));
     CK(cudaGetLastError());
   });
 }
 
-dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
-                                   const void* weight, const void* bias, int param_type,
-                                   int64_t rows, int64_t cols, float eps, int8_t* q, int64_t q_ld,
-                                   float* scale, float* mean, float* rstd, void* stream) {
+dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const dmx_layer_norm_quantize_args* g,
+                                   void* stream) {
   return guarded([&] {
     const char* what = "dmx_layer_norm_quantize";
-    if (!ops) refuse(what, "ops is null");
-    check_shape(what, rows, cols);
+    check_call(what, ops, g);
+    check_shape(what, g->rows, g->cols);
+    const size_t xb = type_bytes(what, "x_type", g->x_type);
     RowArgs a;
-    const size_t xb = type_bytes(what, "x_type", x_type);
-    a.norm = true;
-    a.weight = weight;
-    a.bias = bias;
-    a.param_type = param_type;
-    a.eps = eps;
-    a.mean = mean;
-    a.rstd = rstd;
-    check_norm(what, a);
-    if (rows == 0) return;
-    check_rows(what, "x", x, xb, x_ld, cols);
-    check_rows(what, "q", q, 1, q_ld, cols);
-    check_vector(what, "scale", scale, 4, true);
-    if (static_cast<const void*>(q) == x) refuse(what, "q must not be x");
-    a.x = x;
-    a.x_type = x_type;
-    a.x_ld = x_ld;
-    a.rows = rows;
-    a.cols = (int)cols;
-    a.q = q;
-    a.q_ld = q_ld;
-    a.scale = scale;
+    set_norm(what, g, &a);
+    if (g->rows == 0) return;
+    set_quantized(what, g, xb, &a);
     OnDevice on(ops->device);
     launch_rows(a, static_cast<cudaStream_t>(stream));
     CK(cudaGetLastError());
   });
 }
 
-dmx_status dmx_quantized_linear(dmx_ops* ops, const int8_t* x, int64_t x_ld, const float* x_scale,
-                                const int8_t* w, int64_t w_ld, const float* w_scale,
-                                const float* bias, int64_t rows, int64_t out_features,
-                                int64_t in_features, int activation, const void* residual,
-                                int64_t residual_ld, void* out, int out_type, int64_t out_ld,
-                                void* stream) {
+dmx_status dmx_quantized_linear(dmx_ops* ops, const dmx_quantized_linear_args* g, void* stream) {
   return guarded([&] {
     const char* what = "dmx_quantized_linear";
-    if (!ops) refuse(what, "ops is null");
-    if (rows < 0 || rows > kMaxRows) refuse(what, "rows must be in [0, 2^31 - 1]");
-    if (out_features < 1 || out_features > kMaxCols)
+    check_call(what, ops, g);
+    if (g->rows < 0 || g->rows > kMaxRows) refuse(what, "rows must be in [0, 2^31 - 1]");
+    if (g->out_features < 1 || g->out_features > kMaxCols)
       refuse(what, "out_features must be in [1, 2^29 - 1]");
-    if (in_features < 1 || in_features > kMaxInner)
+    if (g->in_features < 1 || g->in_features > kMaxInner)
       refuse(what, "in_features must be in [1, 131071], the longest exact 32-bit sum");
-    if (activation != DMX_ACT_NONE && activation != DMX_ACT_GELU)
+    if (g->activation != DMX_ACT_NONE && g->activation != DMX_ACT_GELU)
       refuse(what, "activation must be DMX_ACT_NONE or DMX_ACT_GELU");
-    const size_t ob = type_bytes(what, "out_type", out_type);
-    check_vector(what, "x_scale", x_scale, 4, false);
-    check_vector(what, "w_scale", w_scale, 4, false);
-    check_vector(what, "bias", bias, 4, false);
-    if (rows == 0) return;
-    check_rows(what, "x", x, 16, x_ld, in_features);
-    check_rows(what, "w", w, 16, w_ld, in_features);
-    if (x_ld % 16 || w_ld % 16) refuse(what, "x_ld and w_ld must be multiples of 16 bytes");
-    check_rows(what, "out", out, ob, out_ld, out_features);
-    if (residual) {
-      check_rows(what, "residual", residual, ob, residual_ld, out_features);
-      check_in_place(what, residual, out_type, residual_ld, out, out_type, out_ld);
-    }
-    if (out == x || out == w) refuse(what, "out must not be x or w");
+    const size_t ob = type_bytes(what, "out_type", g->out_type);
+    check_vector(what, "x_scale", g->x_scale, 4, false);
+    check_vector(what, "w_scale", g->w_scale, 4, false);
+    check_vector(what, "bias", g->bias, 4, false);
+    if (g->rows == 0) return;
     LinearArgs a;
-    a.x = x;
-    a.x_ld = x_ld;
-    a.x_scale = x_scale;
-    a.w = w;
-    a.w_ld = w_ld;
-    a.w_scale = w_scale;
-    a.bias = bias;
-    a.rows = rows;
-    a.n = (int)out_features;
-    a.k = (int)in_features;
-    a.gelu = activation == DMX_ACT_GELU;
-    a.residual = residual;
-    a.residual_ld = residual_ld;
-    a.out = out;
-    a.out_type = out_type;
-    a.out_ld = out_ld;
+    a.x = g->x;
+    a.x_ld = g->x_ld ? g->x_ld : g->in_features;
+    a.x_scale = g->x_scale;
+    a.w = g->w;
+    a.w_ld = g->w_ld ? g->w_ld : g->in_features;
+    a.w_scale = g->w_scale;
+    a.bias = g->bias;
+    a.rows = g->rows;
+    a.n = (int)g->out_features;
+    a.k = (int)g->in_features;
+    a.gelu = g->activation == DMX_ACT_GELU;
+    a.residual = g->residual;
+    a.residual_ld = g->residual_ld ? g->residual_ld : g->out_features;
+    a.out = g->out;
+    a.out_type = g->out_type;
+    a.out_ld = g->out_ld ? g->out_ld : g->out_features;
     a.err = ops->err;
+    check_rows(what, "x", a.x, 16, a.x_ld, a.k);
+    check_rows(what, "w", a.w, 16, a.w_ld, a.k);
+    if (a.x_ld % 16 || a.w_ld % 16) refuse(what, "x_ld and w_ld must be multiples of 16 bytes");
+    check_rows(what, "out", a.out, ob, a.out_ld, a.n);
+    if (a.residual) {
+      check_rows(what, "residual", a.residual, ob, a.residual_ld, a.n);
+      check_in_place(what, a.residual, a.out_type, a.residual_ld, a.out, a.out_type, a.out_ld);
+    }
+    if (a.out == a.x || a.out == a.w) refuse(what, "out must not be x or w");
     OnDevice on(ops->device);
     if (!launch_quantized_linear(a, static_cast<cudaStream_t>(stream)))
       throw Error(DMX_ERR_CUDA, "dmx_quantized_linear: a tensor map could not be encoded");

@@ -178,7 +178,7 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
 constexpr int kRowsThreads = 256;
 
 template <typename XT, int MODE, int LANES, int NV>
-__global__ void __launch_bounds__(kRowsThreads) rows_warp_kernel(const RowArgs a, bool vec, bool q_vec) {
+__global__ void __launch_bounds__(kRowsThreads) rows_warp_kernel(const RowArgs a, int vec, bool q_vec) {
   const int64_t at = (int64_t)blockIdx.x * (kRowsThreads / LANES) + threadIdx.x / LANES;
   // lanes without a row of their own follow the last one's, for the shuffles
   const bool live = at < a.rows;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_warp_kernel(const RowArgs a
 }
 
 template <typename XT, int MODE, int NV>
-__global__ void __launch_bounds__(1024) rows_block_kernel(const RowArgs a, bool vec, bool q_vec) {
+__global__ void __launch_bounds__(1024) rows_block_kernel(const RowArgs a, int vec, bool q_vec) {
   __shared__ float sh[3][32];
   const Pieces p = {(int)threadIdx.x, (int)blockDim.x, a.cols, vec};
   row_in_registers<XT, MODE, 0, NV>(a, blockIdx.x, true, p, q_vec, sh);
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(1024) rows_block_kernel(const RowArgs a, bool 
 
 // Rows too long for registers: one block re-reads its row for each reduction.
 template <typename XT, int MODE>
-__global__ void __launch_bounds__(1024) rows_long_kernel(const RowArgs a, bool vec, bool q_vec) {
+__global__ void __launch_bounds__(1024) rows_long_kernel(const RowArgs a, int vec, bool q_vec) {
   __shared__ float sh[3][32];
   const RowSum<0> over;
   const Pieces p = {(int)threadIdx.x, (int)blockDim.x, a.cols, vec};
@@ -267,14 +267,14 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(const RowArgs a, bool v
 }
 
 template <typename XT, int MODE, int LANES, int NV>
-void launch_rows_warp(const RowArgs& a, bool vec, bool q_vec, cudaStream_t s) {
+void launch_rows_warp(const RowArgs& a, int vec, bool q_vec, cudaStream_t s) {
   constexpr int per = kRowsThreads / LANES;
   rows_warp_kernel<XT, MODE, LANES, NV>
       <<<(unsigned)((a.rows + per - 1) / per), kRowsThreads, 0, s>>>(a, vec, q_vec);
 }
 
 template <typename XT, int MODE>
-void launch_rows_mode(const RowArgs& a, bool vec, bool q_vec, cudaStream_t s) {
+void launch_rows_mode(const RowArgs& a, int vec, bool q_vec, cudaStream_t s) {
   if (a.cols <= 64) return launch_rows_warp<XT, MODE, 8, 1>(a, vec, q_vec, s);
   if (a.cols <= 128) return launch_rows_warp<XT, MODE, 16, 1>(a, vec, q_vec, s);
   if (a.cols <= 256) return launch_rows_warp<XT, MODE, 32, 1>(a, vec, q_vec, s);
@@ -291,14 +291,17 @@ void launch_rows_mode(const RowArgs& a, bool vec, bool q_vec, cudaStream_t s) {
 
 template <typename XT>
 void launch_rows_typed(const RowArgs& a, cudaStream_t s) {
-  bool vec = rows_on_16(a.x, a.x_ld, sizeof(XT));
-  auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-  if (a.norm) vec = vec && aligned(a.weight) && aligned(a.bias);
+  int vec = vec_of(a.x, a.x_ld, sizeof(XT));
+  auto narrow = [&vec](int other) { vec = std::min(vec, other); };
+  if (a.norm) {
+    narrow(vec_of(a.weight, 0, type_size(a.param_type)));
+    narrow(vec_of(a.bias, 0, type_size(a.param_type)));
+  }
   if (a.y) {
-    vec = vec && rows_on_16(a.y, a.y_ld, type_size(a.y_type));
+    narrow(vec_of(a.y, a.y_ld, type_size(a.y_type)));
     return launch_rows_mode<XT, ROWS_NORM>(a, vec, false, s);
   }
-  vec = vec && aligned(a.col_scale);
+  narrow(vec_of(a.col_scale, 0, 4));
   const bool q_vec = reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.q_ld % 8 == 0;
   if (a.norm) launch_rows_mode<XT, ROWS_NORM_QUANTIZE>(a, vec, q_vec, s);
   else launch_rows_mode<XT, ROWS_QUANTIZE>(a, vec, q_vec, s);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -167,17 +168,11 @@ def lib():
         L.dmx_ops_destroy.argtypes = [vp]
         L.dmx_ops_destroy.restype = None
         L.dmx_ops_check.argtypes = [vp, vp]
-        L.dmx_layer_norm.argtypes = [vp, vp, ci, i64, vp, vp, ci, i64, i64, ctypes.c_float, vp, ci,
-                                     i64, vp, vp, vp]
+        for name in ("dmx_layer_norm", "dmx_layer_norm_backward", "dmx_quantize_rows",
+                     "dmx_layer_norm_quantize", "dmx_quantized_linear"):
+            getattr(L, name).argtypes = [vp, ctypes.c_char_p, vp]
         L.dmx_layer_norm_backward_workspace.argtypes = [i64, i64]
         L.dmx_layer_norm_backward_workspace.restype = ctypes.c_size_t
-        L.dmx_layer_norm_backward.argtypes = [vp, vp, ci, i64, vp, ci, i64, vp, ci, vp, vp, i64,
-                                              i64, vp, i64, vp, vp, vp, ctypes.c_size_t, vp]
-        L.dmx_quantize_rows.argtypes = [vp, vp, ci, i64, vp, i64, i64, vp, i64, vp, vp]
-        L.dmx_layer_norm_quantize.argtypes = [vp, vp, ci, i64, vp, vp, ci, i64, i64,
-                                              ctypes.c_float, vp, i64, vp, vp, vp, vp]
-        L.dmx_quantized_linear.argtypes = [vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, ci, vp,
-                                           i64, vp, ci, i64, vp]
         L.dmx_kernel_launches.restype = ctypes.c_int64
         L.dmx_kernel_launches.argtypes = [ctypes.c_void_p]
         _lib = L
@@ -494,6 +489,16 @@ class Bag:
                                                    None))
 
 
+# The operators' argument structs (dmx_*_args) as bytes, native alignment: one
+# pack and a three-argument call take a third of the time of as many ctypes
+# arguments (0.8 against 2.0 us), which is what a single token's call is made of.
+_LAYER_NORM_ARGS = struct.Struct("@PiqPPiqqfPiqPP").pack
+_LAYER_NORM_BACKWARD_ARGS = struct.Struct("@PiqPiqPiPPqqPqPPPN").pack
+_QUANTIZE_ROWS_ARGS = struct.Struct("@PiqPqqPqP").pack
+_LAYER_NORM_QUANTIZE_ARGS = struct.Struct("@PiqPPiqqfPqPPP").pack
+_QUANTIZED_LINEAR_ARGS = struct.Struct("@PqPPqPPqqqiPqPiq").pack
+
+
 class Ops:
     """The operators on device buffers (dmx_ops_*): layer norm, its backward
     pass, and linear layers on 8-bit integers. Buffers are device pointers
@@ -508,6 +513,9 @@ class Ops:
         h = ctypes.c_void_p()
         _check(L.dmx_ops_create(device, ctypes.byref(h)))
         self._L, self._h, self.device = L, h, device
+        self._layer_norm, self._layer_norm_backward = L.dmx_layer_norm, L.dmx_layer_norm_backward
+        self._quantize_rows, self._layer_norm_quantize = L.dmx_quantize_rows, L.dmx_layer_norm_quantize
+        self._quantized_linear = L.dmx_quantized_linear
 
     def close(self):
         if self._h:
@@ -524,8 +532,9 @@ class Ops:
                    weight: int = 0, bias: int = 0, param_type: int = TYPE_F32, eps: float = 1e-5,
                    x_ld: int = 0, y_ld: int = 0, mean: int = 0, rstd: int = 0, stream: int = 0):
         """y = layer norm of x's rows; ``mean`` and ``rstd`` are kept for the backward pass."""
-        rc = self._L.dmx_layer_norm(self._h, x, x_type, x_ld or cols, weight, bias, param_type, rows,
-                                    cols, eps, y, y_type, y_ld or cols, mean, rstd, stream)
+        rc = self._layer_norm(self._h, _LAYER_NORM_ARGS(
+            x, x_type, x_ld, weight, bias, param_type, rows, cols, eps, y, y_type, y_ld, mean, rstd),
+            stream)
         if rc:
             _check(rc)
 
@@ -539,17 +548,17 @@ class Ops:
                             dweight: int = 0, dbias: int = 0, dy_ld: int = 0, x_ld: int = 0,
                             dx_ld: int = 0, stream: int = 0):
         """dx (x's type), dweight and dbias (float32) of the layer norm; those that are 0 are left out."""
-        rc = self._L.dmx_layer_norm_backward(
-            self._h, dy, dy_type, dy_ld or cols, x, x_type, x_ld or cols, weight, param_type, mean,
-            rstd, rows, cols, dx, dx_ld or cols, dweight, dbias, workspace, workspace_bytes, stream)
+        rc = self._layer_norm_backward(self._h, _LAYER_NORM_BACKWARD_ARGS(
+            dy, dy_type, dy_ld, x, x_type, x_ld, weight, param_type, mean, rstd, rows, cols, dx, dx_ld,
+            dweight, dbias, workspace, workspace_bytes), stream)
         if rc:
             _check(rc)
 
     def quantize_rows(self, x: int, x_type: int, rows: int, cols: int, q: int, scale: int,
                       col_scale: int = 0, x_ld: int = 0, q_ld: int = 0, stream: int = 0):
         """int8 q and one float32 scale per row of x (times ``col_scale``): x ~ q scale."""
-        rc = self._L.dmx_quantize_rows(self._h, x, x_type, x_ld or cols, col_scale, rows, cols, q,
-                                       q_ld or cols, scale, stream)
+        rc = self._quantize_rows(self._h, _QUANTIZE_ROWS_ARGS(
+            x, x_type, x_ld, col_scale, rows, cols, q, q_ld, scale), stream)
         if rc:
             _check(rc)
 
@@ -558,9 +567,9 @@ class Ops:
                             eps: float = 1e-5, x_ld: int = 0, q_ld: int = 0, mean: int = 0,
                             rstd: int = 0, stream: int = 0):
         """layer_norm and quantize_rows in one pass."""
-        rc = self._L.dmx_layer_norm_quantize(self._h, x, x_type, x_ld or cols, weight, bias,
-                                             param_type, rows, cols, eps, q, q_ld or cols, scale,
-                                             mean, rstd, stream)
+        rc = self._layer_norm_quantize(self._h, _LAYER_NORM_QUANTIZE_ARGS(
+            x, x_type, x_ld, weight, bias, param_type, rows, cols, eps, q, q_ld, scale, mean, rstd),
+            stream)
         if rc:
             _check(rc)
 
@@ -570,10 +579,9 @@ class Ops:
                          w_ld: int = 0, residual_ld: int = 0, out_ld: int = 0, stream: int = 0):
         """out = act(x w^T x_scale w_scale + bias) + residual on int8 x and w; their
         pointers and pitches (0 = in_features) are multiples of 16 bytes."""
-        rc = self._L.dmx_quantized_linear(
-            self._h, x, x_ld or in_features, x_scale, w, w_ld or in_features, w_scale, bias, rows,
-            out_features, in_features, activation, residual, residual_ld or out_features, out,
-            out_type, out_ld or out_features, stream)
+        rc = self._quantized_linear(self._h, _QUANTIZED_LINEAR_ARGS(
+            x, x_ld, x_scale, w, w_ld, w_scale, bias, rows, out_features, in_features, activation,
+            residual, residual_ld, out, out_type, out_ld), stream)
         if rc:
             _check(rc)
 

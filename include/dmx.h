@@ -421,8 +421,10 @@ dmx_status dmx_synchronize(dmx_handle* h);
  * in front of it trained afterwards); the reference has no 8-bit path and no
  * gradients, so they replace nothing there.
  *
- * Conventions. Operands are row-major with a pitch (`*_ld`, elements between
- * rows) of at least the row length; rows are tokens. Types are dmx_type, and
+ * Conventions. Each call takes its operands in a struct (zero what is not
+ * given). Operands are row-major with a pitch (`*_ld`, elements between rows; 0
+ * = the row length) of at least the row length; rows are tokens. Types are
+ * dmx_type, and
  * arithmetic is in 32 bits: a 16-bit result is rounded once, when stored.
  * Calls are enqueued on `stream` (a cudaStream_t of the context's device, NULL
  * = legacy default stream), do not wait, allocate nothing and may be captured
@@ -448,10 +450,22 @@ dmx_status dmx_ops_check(dmx_ops* ops, void* stream);
  * `weight` and `bias` (cols values of param_type) may be NULL (1 and 0);
  * `mean` and `rstd` (rows floats each, for the backward pass) may be NULL.
  * In place: y may be x, with x's type and pitch. */
-dmx_status dmx_layer_norm(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
-                          const void* weight, const void* bias, int param_type, int64_t rows,
-                          int64_t cols, float eps, void* y, int y_type, int64_t y_ld, float* mean,
-                          float* rstd, void* stream);
+typedef struct {
+  const void* x;
+  int x_type;
+  int64_t x_ld;
+  const void* weight;
+  const void* bias;
+  int param_type;
+  int64_t rows, cols;
+  float eps;
+  void* y;
+  int y_type;
+  int64_t y_ld;
+  float* mean;
+  float* rstd;
+} dmx_layer_norm_args;
+dmx_status dmx_layer_norm(dmx_ops* ops, const dmx_layer_norm_args* args, void* stream);
 
 /* Its backward pass, from the gradient dy of y and the forward's x, mean and
  * rstd. With h = (x - mean) rstd and g = dy weight:
@@ -464,12 +478,27 @@ dmx_status dmx_layer_norm(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
  * stream has passed it; it may be NULL when neither is wanted. In place: dx
  * may be dy or x, with the same type and pitch. */
 size_t dmx_layer_norm_backward_workspace(int64_t rows, int64_t cols);
-dmx_status dmx_layer_norm_backward(dmx_ops* ops, const void* dy, int dy_type, int64_t dy_ld,
-                                   const void* x, int x_type, int64_t x_ld, const void* weight,
-                                   int param_type, const float* mean, const float* rstd,
-                                   int64_t rows, int64_t cols, void* dx, int64_t dx_ld,
-                                   float* dweight, float* dbias, void* workspace,
-                                   size_t workspace_bytes, void* stream);
+typedef struct {
+  const void* dy;
+  int dy_type;
+  int64_t dy_ld;
+  const void* x;
+  int x_type;
+  int64_t x_ld;
+  const void* weight;
+  int param_type;
+  const float* mean;
+  const float* rstd;
+  int64_t rows, cols;
+  void* dx;
+  int64_t dx_ld;
+  float* dweight;
+  float* dbias;
+  void* workspace;
+  size_t workspace_bytes;
+} dmx_layer_norm_backward_args;
+dmx_status dmx_layer_norm_backward(dmx_ops* ops, const dmx_layer_norm_backward_args* args,
+                                   void* stream);
 
 /* Symmetric 8-bit quantisation with one scale per row. With v = x col_scale
  * (cols floats; NULL = 1), every step rounded to f32:
@@ -477,16 +506,37 @@ dmx_status dmx_layer_norm_backward(dmx_ops* ops, const void* dy, int dy_type, in
  * An all-zero row has scale 0 and q = 0. A row with a NaN has scale NaN, one
  * with an infinity scale infinity, both q = 0, so that a product with them is
  * NaN. Rows of tokens or of a weight matrix (output channels) alike. */
-dmx_status dmx_quantize_rows(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
-                             const float* col_scale, int64_t rows, int64_t cols, int8_t* q,
-                             int64_t q_ld, float* scale, void* stream);
+typedef struct {
+  const void* x;
+  int x_type;
+  int64_t x_ld;
+  const float* col_scale;
+  int64_t rows, cols;
+  int8_t* q;
+  int64_t q_ld;
+  float* scale;
+} dmx_quantize_rows_args;
+dmx_status dmx_quantize_rows(dmx_ops* ops, const dmx_quantize_rows_args* args, void* stream);
 
 /* dmx_layer_norm followed by dmx_quantize_rows, in one pass: y is quantised
  * before it would be rounded to a stored type. */
-dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const void* x, int x_type, int64_t x_ld,
-                                   const void* weight, const void* bias, int param_type,
-                                   int64_t rows, int64_t cols, float eps, int8_t* q, int64_t q_ld,
-                                   float* scale, float* mean, float* rstd, void* stream);
+typedef struct {
+  const void* x;
+  int x_type;
+  int64_t x_ld;
+  const void* weight;
+  const void* bias;
+  int param_type;
+  int64_t rows, cols;
+  float eps;
+  int8_t* q;
+  int64_t q_ld;
+  float* scale;
+  float* mean;
+  float* rstd;
+} dmx_layer_norm_quantize_args;
+dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const dmx_layer_norm_quantize_args* args,
+                                   void* stream);
 
 /* Linear layer on 8-bit integers, one scale per row (token) of x and one per
  * row (output channel) of w (out_features x in_features):
@@ -502,12 +552,23 @@ dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const void* x, int x_type, int6
  * rounding passed straight through) is the same operator: quantise dy with
  * col_scale = w_scale, and multiply by the transposed integers with w_scale
  * NULL. */
-dmx_status dmx_quantized_linear(dmx_ops* ops, const int8_t* x, int64_t x_ld, const float* x_scale,
-                                const int8_t* w, int64_t w_ld, const float* w_scale,
-                                const float* bias, int64_t rows, int64_t out_features,
-                                int64_t in_features, int activation, const void* residual,
-                                int64_t residual_ld, void* out, int out_type, int64_t out_ld,
-                                void* stream);
+typedef struct {
+  const int8_t* x;
+  int64_t x_ld;
+  const float* x_scale;
+  const int8_t* w;
+  int64_t w_ld;
+  const float* w_scale;
+  const float* bias;
+  int64_t rows, out_features, in_features;
+  int activation; /* dmx_activation */
+  const void* residual;
+  int64_t residual_ld;
+  void* out;
+  int out_type;
+  int64_t out_ld;
+} dmx_quantized_linear_args;
+dmx_status dmx_quantized_linear(dmx_ops* ops, const dmx_quantized_linear_args* args, void* stream);
 
 #ifdef __cplusplus
 }
