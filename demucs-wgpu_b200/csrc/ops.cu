@@ -3,8 +3,9 @@
 // and the status codes around the launchers of ops.h. Nothing here throws
 // across the boundary, allocates device memory after dmx_ops_create, or waits
 // (dmx_ops_check excepted), so calls may be captured into a CUDA graph.
-#include <cmath>
+#include <atomic>
 #include <chrono>
+#include <cmath>
 #include <thread>
 
 #include "ops.h"
@@ -16,6 +17,23 @@ struct dmx_ops {
   int device = 0;
   int* err = nullptr;  // raised by a bounded wait that gave up
 };
+
+namespace dmx {
+
+int sm_count() {
+  static std::atomic<int> count[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return 148;
+  int n = count[dev].load();
+  if (n == 0) {
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    count[dev].store(n);
+  }
+  return n;
+}
+
+}  // namespace dmx
 
 namespace {
 

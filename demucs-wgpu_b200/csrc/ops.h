@@ -8,6 +8,9 @@
 
 namespace dmx {
 
+// SMs of the current device.
+int sm_count();
+
 // One pass over rows: optionally the layer norm, then either a store (y) or
 // the 8-bit quantisation (q, scale).
 struct RowArgs {

@@ -35,18 +35,71 @@ DMX_DEVICE void store_from_f32(void* p, int type, int64_t i, float v) {
   else static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
 }
 
-// Eight neighbours at a 16-byte boundary; `wide` (uniform): f32 ones at a
-// 32-byte boundary, in one access. Loads are not through the read-only path: an
-// operator may write its output over its input.
-DMX_DEVICE void load8(const float* p, float* v, bool wide) {
-  if (wide) return ld_global8(p, v);
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// 16- and 32-byte accesses in inline PTX, so that a branch on a type known
+// only at run time stays a branch: the compiler would otherwise run all three
+// types' loads and conversions under predicates (twice the instructions of a
+// bf16 row's arithmetic). Not through the read-only path: an operator may
+// write its output over its input. No "memory" clobber, which made the
+// compiler fetch the launch's arguments anew after every access; the volatile
+// ones keep their order among themselves, and every thread stores only what
+// it has loaded.
+DMX_DEVICE void ld_words4(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "l"(p));
 }
-DMX_DEVICE void load8(const __half* p, float* v, bool) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+DMX_DEVICE void ld_words8(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+                 "=r"(w[7])
+               : "l"(p));
+}
+DMX_DEVICE void st_words4(void* p, const uint32_t* w) {
+  asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]));
+}
+DMX_DEVICE void st_words8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]));
+}
+
+// One element of a cut piece: in PTX too, so that these rare ones are branched over.
+DMX_DEVICE uint32_t ld_bits(const float* p) {
+  uint32_t w;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(w) : "l"(p));
+  return w;
+}
+DMX_DEVICE uint32_t ld_bits(const __half* p) {
+  uint16_t w;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(w) : "l"(p));
+  return w;
+}
+DMX_DEVICE uint32_t ld_bits(const __nv_bfloat16* p) {
+  return ld_bits(reinterpret_cast<const __half*>(p));
+}
+DMX_DEVICE void st_value(float* p, float v) { asm volatile("st.global.f32 [%0], %1;" ::"l"(p), "f"(v)); }
+DMX_DEVICE void st_value(__half* p, __half v) {
+  asm volatile("st.global.u16 [%0], %1;" ::"l"(p), "h"(__half_as_ushort(v)));
+}
+DMX_DEVICE void st_value(__nv_bfloat16* p, __nv_bfloat16 v) {
+  asm volatile("st.global.u16 [%0], %1;" ::"l"(p), "h"(__bfloat16_as_ushort(v)));
+}
+
+// Eight neighbours at a 16-byte boundary as they lie in memory (f32: 8 words,
+// 16-bit types: 4); `wide` (uniform): f32 ones at a 32-byte boundary, in one access.
+DMX_DEVICE void fetch8(const float* p, uint32_t* w, bool wide) {
+  if (wide) return ld_words8(p, w);
+  ld_words4(p, w);
+  ld_words4(p + 4, w + 4);
+}
+DMX_DEVICE void fetch8(const __half* p, uint32_t* w, bool) { ld_words4(p, w); }
+DMX_DEVICE void fetch8(const __nv_bfloat16* p, uint32_t* w, bool) { ld_words4(p, w); }
+
+DMX_DEVICE void unpack8(const uint32_t* w, float* v, float) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+}
+DMX_DEVICE void unpack8(const uint32_t* w, float* v, __half) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -54,19 +107,28 @@ DMX_DEVICE void load8(const __half* p, float* v, bool) {
     v[2 * i + 1] = f.y;
   }
 }
-DMX_DEVICE void load8(const __nv_bfloat16* p, float* v, bool) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+DMX_DEVICE void unpack8(const uint32_t* w, float* v, __nv_bfloat16) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[2 * i] = __uint_as_float(w[i] << 16);
     v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
+// one element in a word of its own
+DMX_DEVICE uint32_t bits_of(float v) { return __float_as_uint(v); }
+DMX_DEVICE uint32_t bits_of(__half v) { return __half_as_ushort(v); }
+DMX_DEVICE uint32_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+DMX_DEVICE float from_bits(uint32_t w, float) { return __uint_as_float(w); }
+DMX_DEVICE float from_bits(uint32_t w, __half) { return __half2float(__ushort_as_half((unsigned short)w)); }
+DMX_DEVICE float from_bits(uint32_t w, __nv_bfloat16) { return __uint_as_float(w << 16); }
+
 DMX_DEVICE void store8(float* p, const float* v, bool wide) {
-  if (wide) return st_global8(p, v);
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+  if (wide) return st_words8(p, w);
+  st_words4(p, w);
+  st_words4(p + 4, w + 4);
 }
 DMX_DEVICE void store8(__half* p, const float* v, bool) {
   uint32_t w[4];
@@ -75,7 +137,7 @@ DMX_DEVICE void store8(__half* p, const float* v, bool) {
     const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  st_words4(p, w);
 }
 DMX_DEVICE void store8(__nv_bfloat16* p, const float* v, bool) {
   uint32_t w[4];
@@ -84,56 +146,84 @@ DMX_DEVICE void store8(__nv_bfloat16* p, const float* v, bool) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  st_words4(p, w);
 }
+
 // How the rows and vectors of a launch may be accessed.
 enum { VEC_NONE = 0, VEC_16 = 1, VEC_32 = 2 };  // by elements; from 16-byte, from 32-byte boundaries
 
 // A row is held by `threads` threads in pieces of eight values. Piece j of
-// thread t is, if every row and vector starts on 16 bytes (`vec`), the eight
+// thread t is, if every row and vector starts on 16 bytes (VEC), the eight
 // neighbours from column (j threads + t) 8 on; else the eight columns
 // (j 8 + e) threads + t, so that a warp's one-element accesses are neighbours.
+template <bool VEC>
 struct Pieces {
-  int t, threads, cols, vec;
+  int t, threads, cols;
+  bool wide;  // VEC: 32-byte boundaries too
   DMX_DEVICE int col(int j, int e) const {
-    return vec ? (j * threads + t) * 8 + e : (j * 8 + e) * threads + t;
+    return VEC ? (j * threads + t) * 8 + e : (j * 8 + e) * threads + t;
   }
   // all eight columns of piece j exist
   DMX_DEVICE bool whole(int j) const { return col(j, 7) < cols; }
   DMX_DEVICE bool has(int j, int e) const { return col(j, e) < cols; }
+  // Some piece of the row (uniform) or piece j may hold only some of its
+  // columns: with VEC, in rows whose length is no multiple of eight.
+  DMX_DEVICE bool ragged() const { return !VEC || (cols & 7); }
+  DMX_DEVICE bool cut(int j) const { return has(j, 0) && !whole(j); }
 
-  // columns past the row's end come as `fill`
+  // Piece j of a row as it lies in memory (VEC: words of the packed values;
+  // else one value a word). Columns past the row's end come as 0.
   template <typename T>
-  DMX_DEVICE void load(const T* p, int j, float* v, float fill = 0.f) const {
-    if (vec && whole(j)) {
-      load8(p + col(j, 0), v, vec == VEC_32);
+  DMX_DEVICE void fetch(const T* p, int j, uint32_t* w) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 0;
+    if (!VEC) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (has(j, e)) w[e] = bits_of(p[col(j, e)]);
+    } else if (whole(j)) {
+      fetch8(p + col(j, 0), w, wide);
+    } else if (cut(j)) {
+      constexpr int kPer = 4 / sizeof(T);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (has(j, e)) w[e / kPer] |= ld_bits(p + col(j, e)) << (e % kPer * 16);
+    }
+  }
+  template <typename T>
+  DMX_DEVICE static void unpack(const uint32_t* w, float* v) {
+    if (VEC) {
+      unpack8(w, v, T());
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = has(j, e) ? to_f32(p[col(j, e)]) : fill;
+      for (int e = 0; e < 8; ++e) v[e] = from_bits(w[e], T());
     }
+  }
+  template <typename T>
+  DMX_DEVICE void load(const T* p, int j, float* v) const {
+    uint32_t w[8];
+    fetch(p, j, w);
+    unpack<T>(w, v);
   }
   template <typename T>
   DMX_DEVICE void store(T* p, int j, const float* v) const {
-    if (vec && whole(j)) {
-      store8(p + col(j, 0), v, vec == VEC_32);
-    } else {
+    if (VEC && whole(j)) {
+      store8(p + col(j, 0), v, wide);
+    } else if (!VEC || cut(j)) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (has(j, e)) p[col(j, e)] = from_f32<T>(v[e]);
+        if (has(j, e)) st_value(p + col(j, e), from_f32<T>(v[e]));
     }
   }
-  // the same for a type known only at run time (uniform over the launch)
-  DMX_DEVICE void load(const void* p, int type, int j, float* v) const {
-    if (type == DMX_TYPE_F32) load(static_cast<const float*>(p), j, v);
-    else if (type == DMX_TYPE_F16) load(static_cast<const __half*>(p), j, v);
-    else load(static_cast<const __nv_bfloat16*>(p), j, v);
-  }
-  DMX_DEVICE void store(void* p, int type, int64_t row0, int j, const float* v) const {
-    if (type == DMX_TYPE_F32) store(static_cast<float*>(p) + row0, j, v);
-    else if (type == DMX_TYPE_F16) store(static_cast<__half*>(p) + row0, j, v);
-    else store(static_cast<__nv_bfloat16*>(p) + row0, j, v);
-  }
 };
+
+// f(T()) for the element type that `type` names (uniform over the launch)
+template <typename F>
+DMX_DEVICE void with_type(int type, F&& f) {
+  if (type == DMX_TYPE_F32) f(float());
+  else if (type == DMX_TYPE_F16) f(__half());
+  else f(__nv_bfloat16());
+}
 
 // The widest access that suits rows of `ld` elements of `bytes` bytes from p
 // on (ld 0: a vector): 16-bit elements need 16 bytes for eight, f32 ones 32.

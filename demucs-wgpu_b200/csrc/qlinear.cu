@@ -582,19 +582,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // host side
 // ---------------------------------------------------------------------------
 
-int sm_count() {
-  static std::atomic<int> count[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return 148;
-  int n = count[dev].load();
-  if (n == 0) {
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    count[dev].store(n);
-  }
-  return n;
-}
-
 // int8 rows: a box of 128 bytes of k by `high` rows; reads past either end give zeros
 bool row_map(CUtensorMap* map, const int8_t* p, int64_t rows, int k, int64_t ld, int high) {
   const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};

@@ -11,11 +11,12 @@
 // with it is NaN; an all-zero row gets scale 0 and q = 0.
 //
 // Bound by HBM: a row is read once, held in registers through its two or three
-// reductions, and written once. Rows of up to 1024 columns belong to a warp
-// (or half or a quarter of one), so nothing waits on other warps and dozens of
-// rows per SM are in flight; up to 16384 columns to a block of as many threads
-// as 16 values each take; longer rows are re-read (from L2) for each
-// reduction.
+// reductions, and written once. Rows of up to 1024 columns (2048 of 16 bits)
+// belong to a warp (or half or a quarter of one), which waits for no other;
+// up to 16384 columns to a block; longer rows are re-read (from L2) for each
+// reduction. 16-bit rows are held as they lie and unpacked in every pass: one
+// more instruction per value and pass, half the registers, and so twice the
+// rows in flight.
 #pragma once
 
 #include <algorithm>
@@ -27,38 +28,70 @@ namespace dmx {
 
 enum { ROWS_NORM = 0, ROWS_NORM_QUANTIZE = 1, ROWS_QUANTIZE = 2 };
 
-// q = rint(v / scale) of a correctly rounded quotient. v times the rounded
-// reciprocal is within 127 * 3 * 2^-24 < 1e-4 of it, so only a product that
-// near a tie needs the division; a subnormal scale, whose reciprocal can
-// overflow, always takes it.
+// max(|a|, |b|, |c|); a NaN among them comes out as a NaN
+DMX_DEVICE float max3_abs(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+
+// q = rint(v / scale) of the correctly rounded quotient: t = v * inv with inv the
+// correctly rounded reciprocal, then one step t + (v - t scale) inv with fused
+// products, which rounds as the quotient does (Markstein 1990) unless the
+// scale's significand is all ones or the remainder underflows; rows with such
+// a scale divide. Every value goes this way: ties are no rarity among 16-bit
+// inputs, whose quotients have few digits, and a branch for values near one
+// took most pieces (112896 x 2048 bf16: 235 us against 165). The integer is
+// read off the sum with 1.5 * 2^23, whose last place is 1; the conversion
+// instructions share the special-function unit, which two of them per value
+// kept busy for longer than the row's memory traffic (316 us).
 struct Quantizer {
   float scale, inv;
   bool usable, divide;
   DMX_DEVICE explicit Quantizer(uint32_t top_bits) {
     scale = __fdiv_rn(__uint_as_float(top_bits), 127.f);
     usable = scale > 0.f && scale < INFINITY;
-    divide = scale < 1.17549435e-38f;
+    // |t| >= 1/4 (less rounds to 0): the remainder's last place is 2^-26 of the scale's
+    divide = scale < 0x1p-100f || (__float_as_uint(scale) & 0x7fffffu) == 0x7fffffu;
     inv = usable && !divide ? __frcp_rn(scale) : 0.f;
   }
-  DMX_DEVICE int operator()(float v) const {
-    if (!usable) return 0;
-    const float t = v * inv;
-    float q = rintf(t);
-    if (divide || fabsf(fabsf(t - q) - 0.5f) < 1e-4f) q = rintf(__fdiv_rn(v, scale));
-    return (int)fminf(fmaxf(q, -127.f), 127.f);
-  }
-  DMX_DEVICE void store(int8_t* row, const Pieces& p, bool vec8, int j, const float* v) const {
-    if (vec8 && p.vec && p.whole(j)) {
-      uint32_t w[2];
+  // eight integers as bytes
+  DMX_DEVICE uint2 operator()(const float* v) const {
+    if (!usable) return make_uint2(0, 0);
+    uint32_t q[8];
+    if (!divide) {
+      const float2 inv2 = make_float2(inv, inv), minus = make_float2(-scale, -scale),
+                   up = make_float2(12582912.f, 12582912.f);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        w[h] = ((uint32_t)(*this)(v[4 * h]) & 255u) | (((uint32_t)(*this)(v[4 * h + 1]) & 255u) << 8) |
-               (((uint32_t)(*this)(v[4 * h + 2]) & 255u) << 16) | ((uint32_t)(*this)(v[4 * h + 3]) << 24);
-      *reinterpret_cast<uint2*>(row + p.col(j, 0)) = make_uint2(w[0], w[1]);
+      for (int e = 0; e < 8; e += 2) {
+        const float2 x = make_float2(v[e], v[e + 1]);
+        float2 t = __fmul2_rn(x, inv2);
+        t = __ffma2_rn(__ffma2_rn(t, minus, x), inv2, t);
+        t = __fadd2_rn(t, up);
+        q[e] = __float_as_uint(t.x);
+        q[e + 1] = __float_as_uint(t.y);
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (p.has(j, e)) row[p.col(j, e)] = (int8_t)(*this)(v[e]);
+        q[e] = (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(v[e], scale)), -127.f), 127.f);
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      w[h] = __byte_perm(__byte_perm(q[4 * h], q[4 * h + 1], 0x0040),
+                         __byte_perm(q[4 * h + 2], q[4 * h + 3], 0x0040), 0x5410);
+    return make_uint2(w[0], w[1]);
+  }
+  template <bool VEC>
+  DMX_DEVICE void store(int8_t* row, const Pieces<VEC>& p, bool q_vec, int j, const float* v) const {
+    const uint2 w = (*this)(v);
+    if (VEC && q_vec && p.whole(j)) {
+      *reinterpret_cast<uint2*>(row + p.col(j, 0)) = w;
+    } else if (p.ragged() || !q_vec) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (p.has(j, e)) row[p.col(j, e)] = (int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
     }
   }
 };
@@ -96,112 +129,204 @@ struct RowSum<0> {
   }
 };
 
-// One row held in NV pieces per thread.
-template <typename XT, int MODE, int LANES, int NV>
-DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const Pieces& p,
+DMX_DEVICE void scale8(float* v, float w) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(w, w));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+DMX_DEVICE void times8(float* v, const float* w) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+DMX_DEVICE void plus8(float* v, const float* w) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+
+DMX_DEVICE void centre8(float* v, float mean) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-mean, -mean));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+// Piece j's values past the row's end become 0.
+template <bool VEC>
+DMX_DEVICE void mask8(const Pieces<VEC>& p, int j, float* v) {
+  if (VEC && !p.has(j, 0)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  } else if (p.ragged()) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = p.has(j, e) ? v[e] : 0.f;
+  }
+}
+
+// One row held in NV pieces per thread; PT is the parameters' type. Without
+// `live` the lanes only take part in the shuffles.
+template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
+DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const Pieces<VEC>& p,
                                  bool q_vec, float (*sh)[32]) {
   const RowSum<LANES> over;
-  const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
-  float v[NV][8];
+  const PT* weight = static_cast<const PT*>(a.weight);
+  const PT* bias = static_cast<const PT*>(a.bias);
+  uint32_t raw[NV][8];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) p.load(x, j, v[j]);
-  if (MODE != ROWS_QUANTIZE) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += v[j][e];
-    const float mean = over.sum(s, sh[0]) / (float)a.cols;
-    s = 0.f;
+  for (int j = 0; j < NV; ++j) p.fetch(static_cast<const XT*>(a.x) + row * a.x_ld, j, raw[j]);
+  auto get = [&](int j, float* v) { Pieces<VEC>::template unpack<XT>(raw[j], v); };
+  float v[8];
+  if (MODE == ROWS_QUANTIZE) {
+    auto value = [&](int j) {
+      get(j, v);
+      if (a.col_scale) {
+        float w[8];
+        p.load(a.col_scale, j, w);
+        times8(v, w);
+      }
+    };
+    float top = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const bool whole = p.whole(j);
+      value(j);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[j][e] = whole || p.has(j, e) ? v[j][e] - mean : 0.f;
-        s = fmaf(v[j][e], v[j][e], s);
-      }
+      for (int e = 0; e < 8; e += 2) top = max3_abs(top, v[e], v[e + 1]);
     }
-    const float rstd = 1.f / sqrtf(over.sum(s, sh[1]) / (float)a.cols + a.eps);
-    if (p.t == 0 && live) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= rstd;
-      if (a.weight) {
-        p.load(a.weight, a.param_type, j, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] *= w[e];
-      }
-      if (a.bias) {
-        p.load(a.bias, a.param_type, j, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] += w[e];
-      }
-    }
-  } else if (a.col_scale) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float w[8];
-      p.load(a.col_scale, j, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= w[e];
-    }
-  }
-  if (MODE == ROWS_NORM) {
+    const Quantizer quant(over.max(__float_as_uint(top), reinterpret_cast<uint32_t*>(sh[2])));
     if (!live) return;
+    if (p.t == 0) a.scale[row] = quant.scale;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) p.store(a.y, a.y_type, row * a.y_ld, j, v[j]);
+    for (int j = 0; j < NV; ++j) {
+      value(j);
+      quant.store(a.q + row * a.q_ld, p, q_vec, j, v);
+    }
     return;
   }
-  // a NaN's bits are above infinity's, so it is kept by the maximum; past the
-  // row's end a NaN mean or rstd must not count
-  uint32_t top = 0;
+  // one piece per thread is the form for a few rows, where a load's latency
+  // counts: the parameters are fetched with the row
+  constexpr bool kEarly = NV == 1;
+  constexpr int kHold = kEarly ? NV : 1;
+  uint32_t wr[kHold][8], br[kHold][8];
+  if (kEarly) {
+    if (weight)
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) p.fetch(weight, j, wr[j]);
+    if (bias)
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) p.fetch(bias, j, br[j]);
+  }
+  float2 s = make_float2(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const bool whole = p.whole(j);
+    get(j, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (whole || p.has(j, e)) top = ::max(top, __float_as_uint(fabsf(v[j][e])));
+    for (int e = 0; e < 8; e += 2) s = __fadd2_rn(s, make_float2(v[e], v[e + 1]));
   }
-  const Quantizer quant(over.max(top, reinterpret_cast<uint32_t*>(sh[2])));
+  const float mean = over.sum(s.x + s.y, sh[0]) / (float)a.cols;
+  s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    get(j, v);
+    centre8(v, mean);
+    mask8(p, j, v);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float2 d = make_float2(v[e], v[e + 1]);
+      s = __ffma2_rn(d, d, s);
+    }
+  }
+  const float rstd = 1.f / sqrtf(over.sum(s.x + s.y, sh[1]) / (float)a.cols + a.eps);
+  if (p.t == 0 && live) {
+    if (a.mean) a.mean[row] = mean;
+    if (a.rstd) a.rstd[row] = rstd;
+  }
+  auto value = [&](int j, float* v) {
+    get(j, v);
+    centre8(v, mean);
+    scale8(v, rstd);
+    float w[8];
+    if (weight) {
+      if (!kEarly) p.fetch(weight, j, wr[0]);
+      Pieces<VEC>::template unpack<PT>(wr[kEarly ? j : 0], w);
+      times8(v, w);
+    }
+    if (bias) {
+      if (!kEarly) p.fetch(bias, j, br[0]);
+      Pieces<VEC>::template unpack<PT>(br[kEarly ? j : 0], w);
+      plus8(v, w);
+    }
+  };
+  if (MODE == ROWS_NORM) {
+    if (!live) return;
+    with_type(a.y_type, [&](auto type) {
+      auto* y = static_cast<decltype(type)*>(a.y) + row * a.y_ld;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        value(j, v);
+        p.store(y, j, v);
+      }
+    });
+    return;
+  }
+  float y[NV][8], top = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    value(j, y[j]);
+    mask8(p, j, y[j]);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) top = max3_abs(top, y[j][e], y[j][e + 1]);
+  }
+  const Quantizer quant(over.max(__float_as_uint(top), reinterpret_cast<uint32_t*>(sh[2])));
   if (!live) return;
   if (p.t == 0) a.scale[row] = quant.scale;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) quant.store(a.q + row * a.q_ld, p, q_vec, j, v[j]);
+  for (int j = 0; j < NV; ++j) quant.store(a.q + row * a.q_ld, p, q_vec, j, y[j]);
 }
 
 constexpr int kRowsThreads = 256;
 
-template <typename XT, int MODE, int LANES, int NV>
-__global__ void __launch_bounds__(kRowsThreads) rows_warp_kernel(const RowArgs a, int vec, bool q_vec) {
-  const int64_t at = (int64_t)blockIdx.x * (kRowsThreads / LANES) + threadIdx.x / LANES;
-  // lanes without a row of their own follow the last one's, for the shuffles
+template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
+__global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
+    rows_warp_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
+  constexpr int per = kRowsThreads / LANES;
+  const int64_t at = (int64_t)blockIdx.x * per + threadIdx.x / LANES;
   const bool live = at < a.rows;
-  const Pieces p = {(int)(threadIdx.x % LANES), LANES, a.cols, vec};
-  row_in_registers<XT, MODE, LANES, NV>(a, live ? at : a.rows - 1, live, p, q_vec, nullptr);
+  // lanes without a row hold nothing
+  const Pieces<VEC> p = {(int)(threadIdx.x % LANES), LANES, live ? a.cols : 0, wide};
+  row_in_registers<XT, PT, MODE, LANES, NV>(a, live ? at : 0, live, p, q_vec, nullptr);
 }
 
-template <typename XT, int MODE, int NV>
-__global__ void __launch_bounds__(1024) rows_block_kernel(const RowArgs a, int vec, bool q_vec) {
+template <typename XT, typename PT, int MODE, int NV, bool VEC>
+__global__ void __launch_bounds__(NV == 4 ? 512 : 1024)
+    rows_block_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
   __shared__ float sh[3][32];
-  const Pieces p = {(int)threadIdx.x, (int)blockDim.x, a.cols, vec};
-  row_in_registers<XT, MODE, 0, NV>(a, blockIdx.x, true, p, q_vec, sh);
+  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
+  row_in_registers<XT, PT, MODE, 0, NV>(a, blockIdx.x, true, p, q_vec, sh);
 }
 
 // Rows too long for registers: one block re-reads its row for each reduction.
-template <typename XT, int MODE>
-__global__ void __launch_bounds__(1024) rows_long_kernel(const RowArgs a, int vec, bool q_vec) {
+template <typename XT, typename PT, int MODE, bool VEC>
+__global__ void __launch_bounds__(1024)
+    rows_long_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
   __shared__ float sh[3][32];
   const RowSum<0> over;
-  const Pieces p = {(int)threadIdx.x, (int)blockDim.x, a.cols, vec};
+  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   const int pieces = (a.cols - 1) / ((int)blockDim.x * 8) + 1;
   const int64_t row = blockIdx.x;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
+  const PT* weight = static_cast<const PT*>(a.weight);
+  const PT* bias = static_cast<const PT*>(a.bias);
   float v[8], w[8], mean = 0.f, rstd = 1.f;
   if (MODE != ROWS_QUANTIZE) {
     float s = 0.f;
@@ -213,9 +338,11 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(const RowArgs a, int ve
     mean = over.sum(s, sh[0]) / (float)a.cols;
     s = 0.f;
     for (int j = 0; j < pieces; ++j) {
-      p.load(x, j, v, mean);
+      p.load(x, j, v);
+      centre8(v, mean);
+      mask8(p, j, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(v[e] - mean, v[e] - mean, s);
+      for (int e = 0; e < 8; ++e) s = fmaf(v[e], v[e], s);
     }
     rstd = 1.f / sqrtf(over.sum(s, sh[1]) / (float)a.cols + a.eps);
     if (threadIdx.x == 0) {
@@ -223,88 +350,94 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(const RowArgs a, int ve
       if (a.rstd) a.rstd[row] = rstd;
     }
   }
-  auto values = [&](int j) {
+  auto value = [&](int j) {
     p.load(x, j, v);
     if (MODE != ROWS_QUANTIZE) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd;
-      if (a.weight) {
-        p.load(a.weight, a.param_type, j, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= w[e];
+      centre8(v, mean);
+      scale8(v, rstd);
+      if (weight) {
+        p.load(weight, j, w);
+        times8(v, w);
       }
-      if (a.bias) {
-        p.load(a.bias, a.param_type, j, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += w[e];
+      if (bias) {
+        p.load(bias, j, w);
+        plus8(v, w);
       }
     } else if (a.col_scale) {
       p.load(a.col_scale, j, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= w[e];
+      times8(v, w);
     }
   };
   if (MODE == ROWS_NORM) {
-    for (int j = 0; j < pieces; ++j) {
-      values(j);
-      p.store(a.y, a.y_type, row * a.y_ld, j, v);
-    }
+    with_type(a.y_type, [&](auto type) {
+      auto* y = static_cast<decltype(type)*>(a.y) + row * a.y_ld;
+      for (int j = 0; j < pieces; ++j) {
+        value(j);
+        p.store(y, j, v);
+      }
+    });
     return;
   }
-  uint32_t top = 0;
+  float top = 0.f;
   for (int j = 0; j < pieces; ++j) {
-    values(j);
+    value(j);
+    mask8(p, j, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (p.has(j, e)) top = ::max(top, __float_as_uint(fabsf(v[e])));
+    for (int e = 0; e < 8; e += 2) top = max3_abs(top, v[e], v[e + 1]);
   }
-  const Quantizer quant(over.max(top, reinterpret_cast<uint32_t*>(sh[2])));
+  const Quantizer quant(over.max(__float_as_uint(top), reinterpret_cast<uint32_t*>(sh[2])));
   if (threadIdx.x == 0) a.scale[row] = quant.scale;
   for (int j = 0; j < pieces; ++j) {
-    values(j);
+    value(j);
     quant.store(a.q + row * a.q_ld, p, q_vec, j, v);
   }
 }
 
-template <typename XT, int MODE, int LANES, int NV>
-void launch_rows_warp(const RowArgs& a, int vec, bool q_vec, cudaStream_t s) {
+template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
+void launch_rows_warp(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   constexpr int per = kRowsThreads / LANES;
-  rows_warp_kernel<XT, MODE, LANES, NV>
-      <<<(unsigned)((a.rows + per - 1) / per), kRowsThreads, 0, s>>>(a, vec, q_vec);
+  rows_warp_kernel<XT, PT, MODE, LANES, NV, VEC>
+      <<<(unsigned)((a.rows + per - 1) / per), kRowsThreads, 0, s>>>(a, wide, q_vec);
 }
 
-template <typename XT, int MODE>
-void launch_rows_mode(const RowArgs& a, int vec, bool q_vec, cudaStream_t s) {
-  if (a.cols <= 64) return launch_rows_warp<XT, MODE, 8, 1>(a, vec, q_vec, s);
-  if (a.cols <= 128) return launch_rows_warp<XT, MODE, 16, 1>(a, vec, q_vec, s);
-  if (a.cols <= 256) return launch_rows_warp<XT, MODE, 32, 1>(a, vec, q_vec, s);
-  if (a.cols <= 512) return launch_rows_warp<XT, MODE, 32, 2>(a, vec, q_vec, s);
-  if (a.cols <= 1024) return launch_rows_warp<XT, MODE, 32, 4>(a, vec, q_vec, s);
-  const unsigned rows = (unsigned)a.rows;
-  if (a.cols > 16384) {
-    rows_long_kernel<XT, MODE><<<rows, 1024, 0, s>>>(a, vec, q_vec);
-    return;
-  }
-  const int threads = ((a.cols + 15) / 16 + 31) / 32 * 32;
-  rows_block_kernel<XT, MODE, 2><<<rows, threads, 0, s>>>(a, vec, q_vec);
+template <typename XT, typename PT, int MODE, int NV, bool VEC>
+void launch_rows_block(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
+  const int threads = ((a.cols + NV * 8 - 1) / (NV * 8) + 31) / 32 * 32;
+  rows_block_kernel<XT, PT, MODE, NV, VEC><<<(unsigned)a.rows, threads, 0, s>>>(a, wide, q_vec);
 }
 
-template <typename XT>
-void launch_rows_typed(const RowArgs& a, cudaStream_t s) {
-  int vec = vec_of(a.x, a.x_ld, sizeof(XT));
-  auto narrow = [&vec](int other) { vec = std::min(vec, other); };
-  if (a.norm) {
-    narrow(vec_of(a.weight, 0, type_size(a.param_type)));
-    narrow(vec_of(a.bias, 0, type_size(a.param_type)));
-  }
+template <typename XT, typename PT, int MODE, bool VEC>
+void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
+  // a few rows: as many threads as there are pieces, for the shortest chain
+  if (a.cols > 256 && a.cols <= 8192 && a.rows <= 2 * sm_count())
+    return launch_rows_block<XT, PT, MODE, 1, VEC>(a, wide, q_vec, s);
+  if (a.cols <= 64) return launch_rows_warp<XT, PT, MODE, 8, 1, VEC>(a, wide, q_vec, s);
+  if (a.cols <= 128) return launch_rows_warp<XT, PT, MODE, 8, 2, VEC>(a, wide, q_vec, s);
+  if (a.cols <= 256) return launch_rows_warp<XT, PT, MODE, 8, 4, VEC>(a, wide, q_vec, s);
+  if (a.cols <= 512) return launch_rows_warp<XT, PT, MODE, 16, 4, VEC>(a, wide, q_vec, s);
+  if (a.cols <= 1024) return launch_rows_warp<XT, PT, MODE, 32, 4, VEC>(a, wide, q_vec, s);
+  if constexpr (sizeof(XT) == 2 && MODE != ROWS_NORM_QUANTIZE && VEC)
+    if (a.cols <= 2048) return launch_rows_warp<XT, PT, MODE, 32, 8, VEC>(a, wide, q_vec, s);
+  constexpr int kBlock = sizeof(XT) == 2 && VEC ? 4 : 2;
+  if (a.cols <= 16384) return launch_rows_block<XT, PT, MODE, kBlock, VEC>(a, wide, q_vec, s);
+  rows_long_kernel<XT, PT, MODE, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a, wide, q_vec);
+}
+
+template <typename XT, typename PT, int MODE>
+void launch_rows_vec(const RowArgs& a, int vec, bool q_vec, cudaStream_t s) {
+  if (vec == VEC_NONE) launch_rows_mode<XT, PT, MODE, false>(a, false, q_vec, s);
+  else launch_rows_mode<XT, PT, MODE, true>(a, vec == VEC_32, q_vec, s);
+}
+
+template <typename XT, typename PT>
+void launch_rows_norm(const RowArgs& a, cudaStream_t s) {
+  int vec = std::min(vec_of(a.x, a.x_ld, sizeof(XT)),
+                     std::min(vec_of(a.weight, 0, sizeof(PT)), vec_of(a.bias, 0, sizeof(PT))));
   if (a.y) {
-    narrow(vec_of(a.y, a.y_ld, type_size(a.y_type)));
-    return launch_rows_mode<XT, ROWS_NORM>(a, vec, false, s);
+    vec = std::min(vec, vec_of(a.y, a.y_ld, type_size(a.y_type)));
+    return launch_rows_vec<XT, PT, ROWS_NORM>(a, vec, false, s);
   }
-  narrow(vec_of(a.col_scale, 0, 4));
-  const bool q_vec = reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.q_ld % 8 == 0;
-  if (a.norm) launch_rows_mode<XT, ROWS_NORM_QUANTIZE>(a, vec, q_vec, s);
-  else launch_rows_mode<XT, ROWS_QUANTIZE>(a, vec, q_vec, s);
+  launch_rows_vec<XT, PT, ROWS_NORM_QUANTIZE>(a, vec, vec_of(a.q, a.q_ld, 1) != VEC_NONE, s);
 }
 
 }  // namespace dmx

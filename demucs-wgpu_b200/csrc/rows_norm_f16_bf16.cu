@@ -1,0 +1,8 @@
+// The layer norm's row kernels (rows.cuh) on f16 rows with bf16 parameters.
+#include "rows.cuh"
+
+namespace dmx {
+
+void launch_rows_norm_f16_bf16(const RowArgs& a, cudaStream_t s) { launch_rows_norm<__half, __nv_bfloat16>(a, s); }
+
+}  // namespace dmx

@@ -1,0 +1,8 @@
+// The layer norm's row kernels (rows.cuh) on f32 rows with f32 parameters.
+#include "rows.cuh"
+
+namespace dmx {
+
+void launch_rows_norm_f32_f32(const RowArgs& a, cudaStream_t s) { launch_rows_norm<float, float>(a, s); }
+
+}  // namespace dmx

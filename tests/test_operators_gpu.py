@@ -475,6 +475,28 @@ def test_quantise_ties_zeros_extremes_and_what_is_not_finite(ops, cols):
     assert np.isnan(scale[[7, 9]]).all() and np.isinf(scale[8]) and not q[[1, 4, 7, 8, 9]].any()
 
 
+@pytest.mark.parametrize("exponent", [-99, -60, 0, 40, 119])
+def test_quantise_next_to_every_tie_of_many_scales(ops, exponent):
+    # the floats around (k + 1/2) scale, for scales of every kind of significand
+    import torch
+
+    rng = np.random.default_rng(100 + exponent)
+    rows = 3000
+    top = np.ldexp(rng.integers(2**23, 2**24, rows).astype(np.float64), exponent - 23).astype(np.float32)
+    ones = np.uint32(0x7FFFFF) | np.uint32((exponent + 127) << 23)  # a scale whose significand is all ones
+    top[:500] = (np.frombuffer(ones.tobytes(), np.float32)[0] * 127.0).astype(np.float32)
+    top[500:900] = np.ldexp(rng.integers(128, 256, 400).astype(np.float64), exponent - 7).astype(np.float32)
+    scale = (top / np.float32(127)).astype(np.float32)
+    k = np.arange(-126, 126) + 0.5
+    near = (k[None, :] * scale[:, None].astype(np.float64)).astype(np.float32)
+    x = np.concatenate([top[:, None], near, np.nextafter(near, np.float32(np.inf)),
+                        np.nextafter(near, np.float32(-np.inf))], axis=1)
+    x = np.clip(x, -top[:, None], top[:, None])
+    q, got = _run_quantise(ops, torch.from_numpy(x).cuda(), None, 0, 0)
+    want_q, want_scale = _quantise_steps(x)
+    assert np.array_equal(got, want_scale) and np.array_equal(q, want_q)
+
+
 @pytest.mark.parametrize("rows,cols,pad", NORM_SHAPES)
 @pytest.mark.parametrize("xt", ["f32", "f16", "bf16"])
 def test_norm_and_quantise_in_one_pass(ops, rows, cols, pad, xt):
