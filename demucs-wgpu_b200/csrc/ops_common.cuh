@@ -122,6 +122,15 @@ DMX_DEVICE float from_bits(uint32_t w, float) { return __uint_as_float(w); }
 DMX_DEVICE float from_bits(uint32_t w, __half) { return __half2float(__ushort_as_half((unsigned short)w)); }
 DMX_DEVICE float from_bits(uint32_t w, __nv_bfloat16) { return __uint_as_float(w << 16); }
 
+// two values in one word, the first in its low half
+DMX_DEVICE uint32_t pack2(float lo, float hi, __half) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+DMX_DEVICE uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 DMX_DEVICE void store8(float* p, const float* v, bool wide) {
   uint32_t w[8];
 #pragma unroll
@@ -130,23 +139,72 @@ DMX_DEVICE void store8(float* p, const float* v, bool wide) {
   st_words4(p, w);
   st_words4(p + 4, w + 4);
 }
-DMX_DEVICE void store8(__half* p, const float* v, bool) {
+template <typename T>
+DMX_DEVICE void store8(T* p, const float* v, bool) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
+  for (int i = 0; i < 4; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1], T());
   st_words4(p, w);
 }
-DMX_DEVICE void store8(__nv_bfloat16* p, const float* v, bool) {
+
+// Four neighbours at a boundary of four elements.
+DMX_DEVICE float4 load4(const float* p) {
   uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
+  ld_words4(p, w);
+  return make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
+                     __uint_as_float(w[3]));
+}
+template <typename T>
+DMX_DEVICE float4 load4(const T* p) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+  float v[8];
+  unpack8(w, v, T());
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+DMX_DEVICE void store4(float* p, float4 v) {
+  const uint32_t w[4] = {__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z),
+                         __float_as_uint(v.w)};
   st_words4(p, w);
+}
+template <typename T>
+DMX_DEVICE void store4(T* p, float4 v) {
+  asm volatile("st.global.v2.b32 [%0], {%1, %2};" ::"l"(p), "r"(pack2(v.x, v.y, T())),
+               "r"(pack2(v.z, v.w, T())));
+}
+
+// Eight values, two to an instruction.
+DMX_DEVICE void scale8(float* v, float w) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(w, w));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+DMX_DEVICE void times8(float* v, const float* w) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+DMX_DEVICE void plus8(float* v, const float* w) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
+}
+DMX_DEVICE void centre8(float* v, float mean) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-mean, -mean));
+    v[e] = r.x;
+    v[e + 1] = r.y;
+  }
 }
 
 // How the rows and vectors of a launch may be accessed.

@@ -35,16 +35,63 @@ constexpr uint32_t i8_idesc(int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-template <typename OT, bool GELU>
-DMX_DEVICE float activate(float v) {
-  return GELU ? gelu(v) : v;
+// max that keeps a NaN
+DMX_DEVICE float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
 
-// One output from its exact sum: scales in the order row, channel, then the
-// bias in the same rounding as the last product.
-template <typename OT, bool GELU>
+// GELU of 2 P values: z (1 + erf(z / sqrt 2)) / 2 = max(z, 0) + n E(n) with
+// n = -|z| and E(n) = erfc(-n / sqrt 2) / 2 = exp(-n^2 / 2) R(n). R is smooth (a
+// scaled complementary error function); this polynomial of degree 10 is the
+// minimax fit of exp(-n^2 / 2) R(n) on [-4.5, 0], found by linear programming
+// on 4000 Chebyshev points, off by at most 3.8e-8 there (1.9e-7 |z| with f32's
+// roundings; erff's own form: 1.2e-7 |z|). Past 4.5 the exponential falls faster
+// than the polynomial grows; past 16 it is 0 and n stays there, so that nothing
+// overflows. -infinity gives 0, a NaN stays one. One special-function operation
+// and paired FMAs a value; each step for all the pairs before the next, so
+// that a coefficient is set up once.
+template <int P>
+DMX_DEVICE void gelu_pairs(float2* z) {
+  constexpr float kR[11] = {0.49999997f,    0.39893848f,   0.24993826f,   0.13261056f,
+                            0.06137684f,    0.024601875f,  0.0081619099f, 0.0020786086f,
+                            0.00036845609f, 3.9511244e-05f, 1.9008927e-06f};
+  float2 n[P], r[P], e[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    n[i] = make_float2(max_nan(-fabsf(z[i].x), -16.f), max_nan(-fabsf(z[i].y), -16.f));
+    r[i] = make_float2(kR[10], kR[10]);
+  }
+#pragma unroll
+  for (int k = 9; k >= 0; --k)
+#pragma unroll
+    for (int i = 0; i < P; ++i) r[i] = __ffma2_rn(r[i], n[i], make_float2(kR[k], kR[k]));
+  // exp(-n^2 / 2) = 2^(-n^2 log2(e) / 2)
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    e[i] = __fmul2_rn(__fmul2_rn(n[i], n[i]), make_float2(-0.72134752f, -0.72134752f));
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i].x) : "f"(e[i].x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i].y) : "f"(e[i].y));
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    z[i] = __ffma2_rn(n[i], __fmul2_rn(r[i], e[i]),
+                      make_float2(fmaxf(z[i].x, 0.f), fmaxf(z[i].y, 0.f)));
+}
+
+// Outputs of one row from their exact sums: scales in the order row, channel,
+// then the bias in the same rounding as the last product.
+DMX_DEVICE float2 scaled2(int acc0, int acc1, float xs, float2 ws, float2 b) {
+  return __ffma2_rn(__fmul2_rn(make_float2((float)acc0, (float)acc1), make_float2(xs, xs)), ws, b);
+}
+template <bool GELU>
 DMX_DEVICE float linear_value(int acc, float xs, float ws, float b) {
-  return activate<OT, GELU>(fmaf((float)acc * xs, ws, b));
+  float2 v = scaled2(acc, acc, xs, make_float2(ws, ws), make_float2(b, b));
+  if (GELU) gelu_pairs<1>(&v);
+  return v.x;
 }
 
 template <typename OT>
@@ -128,7 +175,7 @@ __global__ void __launch_bounds__(kGemvThreads) linear_gemv_kernel(const LinearA
     int t = 0;
     for (int p = 0; p < kw; ++p) t += part[g * kw + p][e];
     store_out<OT>(a, m, n,
-                  linear_value<OT, GELU>(t, a.x_scale ? a.x_scale[m] : 1.f,
+                  linear_value<GELU>(t, a.x_scale ? a.x_scale[m] : 1.f,
                                          a.w_scale ? a.w_scale[n] : 1.f, a.bias ? a.bias[n] : 0.f));
   }
 }
@@ -302,7 +349,7 @@ __global__ void __launch_bounds__(kFewThreads)
     const int n = n0 + c;
     const int64_t row = m0 + m;
     store_out<OT>(a, row, n,
-                  linear_value<OT, GELU>(acc, a.x_scale ? a.x_scale[row] : 1.f,
+                  linear_value<GELU>(acc, a.x_scale ? a.x_scale[row] : 1.f,
                                          a.w_scale ? a.w_scale[n] : 1.f, a.bias ? a.bias[n] : 0.f));
   }
   // a peer may still be reading this CTA's partial sums
@@ -319,104 +366,69 @@ __global__ void __launch_bounds__(kFewThreads)
 // more rows: persistent 128 x BN tiles
 // ---------------------------------------------------------------------------
 
-constexpr int kTileThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
-constexpr int kEpiThreads = 256;
 constexpr int kGroupRows = 8;  // row tiles per group of the tile order
 
+// Warp 0 issues TMA, warp 1 the MMAs, the others are the epilogue: four, one
+// per quarter of the accumulator's lanes, for every 64 columns.
 template <int BN>
-struct TileSmem {
+struct Tile {
+  static constexpr int EPI_WARPS = BN / 16, THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int A = 128 * kBlockK, B = BN * kBlockK, STAGE = A + B;
-  static constexpr int STAGES = 192 * 1024 / STAGE;
-  static constexpr int COLUMN = 2 * BN * 8;             // two tiles' (w_scale, bias) pairs
-  static constexpr int TURN = (kEpiThreads / 32) * 32 * 17 * 4;  // epilogue warps' transposes
-  static constexpr int TOTAL = STAGES * STAGE + COLUMN + TURN + 1024 + 256;
+  static constexpr int TURN = EPI_WARPS * 4096;       // epilogue warps' outputs on their way
+  static constexpr int COLUMN = EPI_WARPS * 64 * 8;   // their channel scales and biases
+  static constexpr int STAGES = (227 * 1024 - TURN - COLUMN - 1024 - 256) / STAGE;
+  static constexpr int TOTAL = STAGES * STAGE + TURN + COLUMN + 1024 + 256;
   static constexpr uint32_t COLS = 2 * BN;
 };
 
 // Tile t of the order: groups of kGroupRows row tiles, row tile fastest, so
 // the CTAs at work together share both operands' tiles in L2.
-DMX_DEVICE void tile_at(int64_t t, int64_t mtiles, int ntiles, int64_t& m0, int& n_tile) {
-  const int64_t per = (int64_t)kGroupRows * ntiles, g = t / per;
-  const int64_t in_group = t - g * per;
-  const int high = (int)min((int64_t)kGroupRows, mtiles - g * kGroupRows);
-  n_tile = (int)(in_group / high);
-  m0 = (g * kGroupRows + in_group % high) * 128;
-}
+struct TileOrder {
+  uint32_t mtiles, ntiles, total;
+  DMX_DEVICE void at(uint32_t t, int64_t& m0, int& n_tile) const {
+    const uint32_t per = kGroupRows * ntiles, g = t / per, in_group = t - g * per;
+    const uint32_t high = min((uint32_t)kGroupRows, mtiles - g * kGroupRows);
+    n_tile = (int)(in_group / high);
+    m0 = (int64_t)(g * kGroupRows + in_group % high) * 128;
+  }
+};
 
+// One epilogue warp's 32 rows x 64 columns of a tile, a lane holding a row,
+// to memory by whole 128-byte lines: through 4 KB of shared memory in which the
+// 16-byte units of row r are permuted by r % 8, so that neither the rows'
+// writes nor the lines' reads meet in a bank. (Stores of 32 bytes to each of 32
+// rows ran at 2.1 TB/s for 16-bit outputs, 2.9 for f32 ones.)
 template <typename OT>
-struct Pack;  // 16 values of a row as 32-byte accesses
-template <>
-struct Pack<float> {
-  static DMX_DEVICE void store(float* p, const float* v) {
-    st_global8(p, v);
-    st_global8(p + 8, v + 8);
+struct Lines {
+  unsigned char* buf;  // 32 rows of 128 bytes
+  int lane;
+  DMX_DEVICE void* unit(int row, int u) const { return buf + row * 128 + ((u ^ (row & 7)) << 4); }
+  // 8 / 4 values of this lane's row as unit u
+  DMX_DEVICE void put_packed(int u, const float* v) const {
+    *reinterpret_cast<uint4*>(unit(lane, u)) =
+        make_uint4(pack2(v[0], v[1], OT()), pack2(v[2], v[3], OT()), pack2(v[4], v[5], OT()),
+                   pack2(v[6], v[7], OT()));
   }
-  static DMX_DEVICE void load(const float* p, float* v) {
-    ld_global8(p, v);
-    ld_global8(p + 8, v + 8);
-  }
-};
-template <>
-struct Pack<__half> {
-  static DMX_DEVICE void store(__half* p, const float* v) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    st_global8(reinterpret_cast<uint32_t*>(p), w);
-  }
-  static DMX_DEVICE void load(const __half* p, float* v) {
-    float w[8];
-    ld_global8(reinterpret_cast<const float*>(p), w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __float_as_uint(w[i]);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-};
-template <>
-struct Pack<__nv_bfloat16> {
-  static DMX_DEVICE void store(__nv_bfloat16* p, const float* v) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    st_global8(reinterpret_cast<uint32_t*>(p), w);
-  }
-  static DMX_DEVICE void load(const __nv_bfloat16* p, float* v) {
-    float w[8];
-    ld_global8(reinterpret_cast<const float*>(p), w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __float_as_uint(w[i]);
-      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
+  DMX_DEVICE void put_f32(int u, const float* v) const {
+    *reinterpret_cast<float4*>(unit(lane, u)) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
 
 template <int BN, typename OT, bool GELU>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tm_x,
-                       const __grid_constant__ CUtensorMap tm_w, const LinearArgs a,
-                       int64_t mtiles, int ntiles, int wide) {
-  using S = TileSmem<BN>;
+                       const __grid_constant__ CUtensorMap tm_w,
+                       const __grid_constant__ LinearArgs a,
+                       const __grid_constant__ TileOrder order, int wide) {
+  using S = Tile<BN>;
   constexpr int STAGES = S::STAGES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float2* column = reinterpret_cast<float2*>(smem + STAGES * S::STAGE);  // [2][BN]
-  float* turn = reinterpret_cast<float*>(smem + STAGES * S::STAGE + S::COLUMN);
+  unsigned char* turn = smem + STAGES * S::STAGE;
+  float4* column = reinterpret_cast<float4*>(turn + S::TURN);
   Pipe pipe;
-  pipe.full = reinterpret_cast<uint64_t*>(smem + STAGES * S::STAGE + S::COLUMN + S::TURN);
+  pipe.full = reinterpret_cast<uint64_t*>(turn + S::TURN + S::COLUMN);
   pipe.empty = pipe.full + STAGES;
   uint64_t* acc_full = pipe.empty + STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2]
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpiThreads);
+      mbar_init(&acc_empty[i], 32 * S::EPI_WARPS);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -441,17 +453,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   tc_after_sync();
   const uint32_t tmem = *slot;
-  const int64_t total = mtiles * ntiles;
   const int blocks = (a.k + kBlockK - 1) / kBlockK;
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (uint32_t t = blockIdx.x; t < order.total && ok; t += gridDim.x) {
         int64_t m0;
         int nt;
-        tile_at(t, mtiles, ntiles, m0, nt);
+        order.at(t, m0, nt);
         for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 21)) {
@@ -471,7 +482,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       uint32_t it = 0;
       int tl = 0;
       bool ok = true;
-      for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x, ++tl) {
+      for (uint32_t t = blockIdx.x; t < order.total && ok; t += gridDim.x, ++tl) {
         const int acc = tl & 1;
         if (!mbar_wait(&acc_empty[acc], ((tl >> 1) & 1) ^ 1, a.err, 22)) {
           ok = false;
@@ -495,73 +506,128 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!ok) drain_mmas(drain, a.err);
     }
   } else {
-    // two warps per quarter of the accumulator's lanes (rows); half hh takes
-    // the 32-column chunks 64 j + 32 hh
-    const int e = threadIdx.x - 64, quarter = warp % 4, hh = (warp - 2) / 4;
+    // this warp: rows 32 quarter + lane, columns c_lo .. c_lo + 63 of each tile
+    const int quarter = warp % 4, c_lo = (warp - 2) / 4 * 64;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    float* mine = turn + (warp - 2) * 32 * 17;
+    const Lines<OT> lines = {turn + (warp - 2) * 4096, lane};
+    // its channel scales and biases, two columns to 16 bytes. A tile's are
+    // fetched while the tile before it is worked on, each warp its own: no
+    // barrier among the epilogue's warps, which so drift apart and share the
+    // issue slots with one another's waits.
+    float4* col = column + (warp - 2) * 32;
+    float4 sb;
+    float xs;
+    int64_t m0_next;
+    int nt_next;
+    auto fetch = [&](uint32_t t) {
+      order.at(t, m0_next, nt_next);
+      const int n = nt_next * BN + c_lo + 2 * lane;
+      sb = make_float4(1.f, 1.f, 0.f, 0.f);
+      if (a.w_scale) {
+        if (n < a.n) sb.x = a.w_scale[n];
+        if (n + 1 < a.n) sb.y = a.w_scale[n + 1];
+      }
+      if (a.bias) {
+        if (n < a.n) sb.z = a.bias[n];
+        if (n + 1 < a.n) sb.w = a.bias[n + 1];
+      }
+      const int64_t m = m0_next + quarter * 32 + lane;
+      xs = m < a.rows && a.x_scale ? a.x_scale[m] : 1.f;
+    };
     bool ok = true;
     int tl = 0;
-    for (int64_t t = blockIdx.x; t < total; t += gridDim.x, ++tl) {
-      int64_t m0;
-      int nt;
-      tile_at(t, mtiles, ntiles, m0, nt);
-      const int n0 = nt * BN, acc = tl & 1;
-      float2* col = column + acc * BN;
-      // this tile's channel scales and biases; the other buffer is still read
-      for (int c = e; c < BN; c += kEpiThreads) {
-        const int n = n0 + c;
-        col[c] = make_float2(n < a.n && a.w_scale ? a.w_scale[n] : 1.f,
-                             n < a.n && a.bias ? a.bias[n] : 0.f);
-      }
-      const int64_t m = m0 + quarter * 32 + lane;
-      const float xs = m < a.rows && a.x_scale ? a.x_scale[m] : 1.f;
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+    if (blockIdx.x < order.total) fetch(blockIdx.x);
+    for (uint32_t t = blockIdx.x; t < order.total; t += gridDim.x, ++tl) {
+      const int64_t m0 = m0_next;
+      const int n0 = nt_next * BN, acc = tl & 1;
+      const float row_scale = xs;
+      __syncwarp();
+      col[lane] = sb;
+      __syncwarp();
+      if (t + gridDim.x < order.total) fetch(t + gridDim.x);
       if (ok && !mbar_wait(&acc_full[acc], (tl >> 1) & 1, a.err, 24)) ok = false;
       // the lanes may end a wait that gave up apart
       ok = __all_sync(0xffffffffu, ok);
       tc_after_sync();
       if (ok) {
+        const int rows = (int)min((int64_t)32, a.rows - m0 - quarter * 32);
+        // columns of one pass through the lines: 16-bit outputs go rounded, 64 to
+        // a line; where a residual is added first they go as f32, as f32 ones do
+        const bool packed = sizeof(OT) == 2 && !a.residual;
 #pragma unroll 1
-        for (int c0 = hh * 32; c0 < BN && n0 + c0 < a.n; c0 += 64) {
-          uint32_t r[32];
-          tmem_ld32_nw(tmem + lanes + (uint32_t)(acc * BN + c0), r);
-          tmem_ld_wait<32>(r);
+        for (int c0 = c_lo; c0 < c_lo + 64 && n0 + c0 < a.n; c0 += 16) {
+          uint32_t r[16];
+          tmem_ld16_nw(tmem + lanes + (uint32_t)(acc * BN + c0), r);
+          tmem_ld_wait<16>(r);
+          float2 v2[8];
 #pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            const int n = n0 + c0 + h;
-            if (n >= a.n) break;
-            float v[16];
+          for (int i = 0; i < 8; ++i) {
+            const float4 q = col[(c0 - c_lo) / 2 + i];
+            v2[i] = scaled2((int)r[2 * i], (int)r[2 * i + 1], row_scale, make_float2(q.x, q.y),
+                            make_float2(q.z, q.w));
+          }
+          if (GELU) gelu_pairs<8>(v2);
+          float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 sb = *reinterpret_cast<const float4*>(col + c0 + h + i);
-              v[i] = linear_value<OT, GELU>((int)r[h + i], xs, sb.x, sb.y);
-              v[i + 1] = linear_value<OT, GELU>((int)r[h + i + 1], xs, sb.z, sb.w);
-            }
-            if (wide && n + 16 <= a.n) {
-              if (m < a.rows) {
-                if (a.residual) {
-                  float q[16];
-                  Pack<OT>::load(static_cast<const OT*>(a.residual) + m * a.residual_ld + n, q);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) v[i] += q[i];
-                }
-                Pack<OT>::store(static_cast<OT*>(a.out) + m * a.out_ld + n, v);
-              }
-            } else {
-              // rows that do not start on 32 bytes: turned in shared memory, so
-              // that a store covers neighbouring columns of two rows
-#pragma unroll
-              for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = v[i];
-              __syncwarp();
-              const int c = lane & 15;
-              for (int i = lane >> 4; i < 32; i += 2) {
-                const int64_t row = m0 + quarter * 32 + i;
-                if (row < a.rows && n + c < a.n) store_out<OT>(a, row, n + c, mine[i * 17 + c]);
-              }
-              __syncwarp();
+          for (int i = 0; i < 8; ++i) {
+            v[2 * i] = v2[i].x;
+            v[2 * i + 1] = v2[i].y;
+          }
+          if constexpr (sizeof(OT) == 2) {
+            if (packed) {
+              lines.put_packed((c0 & 63) / 8, v);
+              lines.put_packed((c0 & 63) / 8 + 1, v + 8);
             }
           }
+          if (!packed) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lines.put_f32((c0 & 31) / 4 + i, v + 4 * i);
+          }
+          // the pass is full, or the matrix ends here
+          const int span = packed ? 64 : 32, first = c0 & ~(span - 1);
+          if ((c0 & (span - 1)) + 16 < span && n0 + c0 + 16 < a.n) continue;
+          __syncwarp();
+          const int n = n0 + first, cols = min(span, a.n - n);
+          OT* out = static_cast<OT*>(a.out) + (m0 + quarter * 32) * a.out_ld + n;
+          const OT* residual = static_cast<const OT*>(a.residual) +
+                               (m0 + quarter * 32) * a.residual_ld + n;
+          if (packed && wide && cols == 64) {
+            if constexpr (sizeof(OT) == 2) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int row = 4 * i + lane / 8;
+                const uint4 w = *reinterpret_cast<const uint4*>(lines.unit(row, lane & 7));
+                if (row < rows)
+                  st_words4(out + row * a.out_ld + (lane & 7) * 8, reinterpret_cast<const uint32_t*>(&w));
+              }
+            }
+          } else if (!packed && wide && cols == 32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = 4 * i + lane / 8;
+              float4 f = *reinterpret_cast<const float4*>(lines.unit(row, lane & 7));
+              if (row < rows) {
+                if (a.residual) {
+                  const float4 q = load4(residual + row * a.residual_ld + (lane & 7) * 4);
+                  f = make_float4(f.x + q.x, f.y + q.y, f.z + q.z, f.w + q.w);
+                }
+                store4(out + row * a.out_ld + (lane & 7) * 4, f);
+              }
+            }
+          } else {
+            // rows that do not start on 16 bytes, or end in this pass: by elements
+            for (int row = 0; row < rows; ++row)
+              for (int c = lane; c < cols; c += 32) {
+                float f;
+                if (packed)
+                  f = to_f32(static_cast<const OT*>(lines.unit(row, c / 8))[c % 8]);
+                else
+                  f = static_cast<const float*>(lines.unit(row, c / 4))[c % 4];
+                if (a.residual) f += to_f32(residual[row * a.residual_ld + c]);
+                out[row * a.out_ld + c] = from_f32<OT>(f);
+              }
+          }
+          __syncwarp();
         }
       }
       tc_before_sync();
@@ -633,18 +699,18 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
   CUtensorMap tw, tx;
   if (!row_map(&tx, a.x, a.rows, a.k, a.x_ld, 128) || !row_map(&tw, a.w, a.n, a.k, a.w_ld, BN))
     return false;
-  using S = TileSmem<BN>;
+  using S = Tile<BN>;
   auto kernel = linear_tile_kernel<BN, OT, GELU>;
   static PerDevice once;
   if (once.first()) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
-  const int64_t mtiles = (a.rows + 127) / 128;
-  const int ntiles = (a.n + BN - 1) / BN;
-  const size_t pitch = sizeof(OT);
-  const bool wide = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_ld * pitch % 32 == 0 &&
-                    (!a.residual || (reinterpret_cast<uintptr_t>(a.residual) % 32 == 0 &&
-                                     a.residual_ld * pitch % 32 == 0));
+  const int64_t mtiles = (a.rows + 127) / 128, ntiles = (a.n + BN - 1) / BN;
+  if (mtiles * ntiles > INT32_MAX) return false;  // no memory holds such an output
+  const TileOrder order = {(uint32_t)mtiles, (uint32_t)ntiles, (uint32_t)(mtiles * ntiles)};
+  const int pitch = sizeof(OT);
+  const bool wide = vec_of(a.out, a.out_ld, pitch) != VEC_NONE &&
+                    (!a.residual || vec_of(a.residual, a.residual_ld, pitch) != VEC_NONE);
   const unsigned grid = (unsigned)std::min<int64_t>(mtiles * ntiles, sm_count());
-  kernel<<<grid, kTileThreads, S::TOTAL, s>>>(tx, tw, a, mtiles, ntiles, wide ? 1 : 0);
+  kernel<<<grid, S::THREADS, S::TOTAL, s>>>(tx, tw, a, order, wide ? 1 : 0);
   return true;
 }
 
@@ -663,10 +729,14 @@ bool launch_typed(const LinearArgs& a, cudaStream_t s) {
     if (a.rows <= 64) return launch_few<64, 4, OT, GELU>(a, s);
     return launch_few<128, 3, OT, GELU>(a, s);
   }
-  // the widest tile that still gives every SM one
-  const int64_t mtiles = (a.rows + 127) / 128;
-  if (mtiles * ((a.n + 255) / 256) >= sm_count()) return launch_tile<256, OT, GELU>(a, s);
-  if (mtiles * ((a.n + 127) / 128) >= sm_count()) return launch_tile<128, OT, GELU>(a, s);
+  // the tile width whose rounds over the SMs take least: a tile costs its
+  // columns and about 32 more for its start and end
+  const int64_t mtiles = (a.rows + 127) / 128, sms = sm_count();
+  auto cost = [&](int bn) {
+    return (mtiles * ((a.n + bn - 1) / bn) + sms - 1) / sms * (bn + 32);
+  };
+  if (cost(256) <= cost(128) && cost(256) <= cost(64)) return launch_tile<256, OT, GELU>(a, s);
+  if (cost(128) <= cost(64)) return launch_tile<128, OT, GELU>(a, s);
   return launch_tile<64, OT, GELU>(a, s);
 }
 

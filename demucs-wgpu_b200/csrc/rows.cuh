@@ -129,39 +129,6 @@ struct RowSum<0> {
   }
 };
 
-DMX_DEVICE void scale8(float* v, float w) {
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(w, w));
-    v[e] = r.x;
-    v[e + 1] = r.y;
-  }
-}
-DMX_DEVICE void times8(float* v, const float* w) {
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
-    v[e] = r.x;
-    v[e + 1] = r.y;
-  }
-}
-DMX_DEVICE void plus8(float* v, const float* w) {
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
-    v[e] = r.x;
-    v[e + 1] = r.y;
-  }
-}
-
-DMX_DEVICE void centre8(float* v, float mean) {
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-mean, -mean));
-    v[e] = r.x;
-    v[e + 1] = r.y;
-  }
-}
 // Piece j's values past the row's end become 0.
 template <bool VEC>
 DMX_DEVICE void mask8(const Pieces<VEC>& p, int j, float* v) {
