@@ -30,9 +30,19 @@ DMX_DEVICE void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
-// s32 accumulator, s8 operands, both K-major, 128 x n
-constexpr uint32_t i8_idesc(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+// The same by a pair of CTAs: rows 0..127 of D and A in the first's memory,
+// 128..255 in the second's, B's rows in halves likewise.
+DMX_DEVICE void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// s32 accumulator, s8 operands, both K-major, m x n
+constexpr uint32_t i8_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // max that keeps a NaN
@@ -196,20 +206,76 @@ DMX_DEVICE void drain_loads(const Pipe& p, uint32_t issued, int* err) {
   for (uint32_t it = issued > STAGES ? issued - STAGES : 0; it < issued; ++it)
     mbar_wait(&p.full[it % STAGES], (it / STAGES) & 1, err, 14);
 }
-// The same for the MMAs issued so far.
+// A barrier of both CTAs of a pair gets an arrival once the pair's MMAs so far are done.
+DMX_DEVICE void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+template <bool PAIR>
+DMX_DEVICE void commit(uint64_t* bar) {
+  if (PAIR) umma_commit_pair(bar);
+  else umma_commit(bar);
+}
+// As drain_loads, for the MMAs issued so far.
+template <bool PAIR>
 DMX_DEVICE void drain_mmas(uint64_t* bar, int* err) {
-  umma_commit(bar);
+  commit<PAIR>(bar);
   mbar_wait(bar, 0, err, 15);
 }
-
-DMX_DEVICE void tmem_alloc(uint32_t* slot, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(slot)),
-               "r"(cols));
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// Shared memory of CTA `rank` of the cluster at this CTA's address p.
+DMX_DEVICE uint32_t of_rank(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
 }
+DMX_DEVICE void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A tile into this CTA's memory, its bytes counted at the first CTA's barrier.
+DMX_DEVICE void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+template <bool PAIR>
+DMX_DEVICE void tmem_alloc(uint32_t* slot, uint32_t cols) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(slot)),
+                 "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(slot)),
+                 "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+}
+template <bool PAIR>
 DMX_DEVICE void tmem_free(uint32_t tmem, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+}
+DMX_DEVICE bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+// A bounded wait of a whole warp, whose lanes may end one that gives up apart.
+DMX_DEVICE bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
 DMX_DEVICE void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 DMX_DEVICE void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -221,13 +287,15 @@ DMX_DEVICE void cluster_sync() {
 
 // The MMAs of one landed stage: `left` bytes of k, 32 per instruction (the
 // rest of a last stage was filled with zeros).
-template <int N>
+template <int N, bool PAIR>
 DMX_DEVICE void mma_stage(uint32_t d, uint32_t a_addr, uint32_t b_addr, int left, bool first) {
 #pragma unroll
   for (int j = 0; j < kBlockK / 32; ++j)
-    if (j * 32 < left)
-      umma_i8(d, umma_desc_k(a_addr + j * 32, 128), umma_desc_k(b_addr + j * 32, 128), i8_idesc(N),
-              !(first && j == 0));
+    if (j * 32 < left) {
+      const uint64_t ad = umma_desc_k(a_addr + j * 32, 128), bd = umma_desc_k(b_addr + j * 32, 128);
+      if (PAIR) umma_i8_pair(d, ad, bd, i8_idesc(256, N), !(first && j == 0));
+      else umma_i8(d, ad, bd, i8_idesc(128, N), !(first && j == 0));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -275,7 +343,7 @@ __global__ void __launch_bounds__(kFewThreads)
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(slot, S::COLS);
+  if (warp == 1) tmem_alloc<false>(slot, S::COLS);
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
@@ -299,10 +367,10 @@ __global__ void __launch_bounds__(kFewThreads)
       if (!mbar_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 12)) break;
       tc_after_sync();
       const uint32_t addr = smem_u32(smem + s * S::STAGE);
-      mma_stage<BT>(tmem, addr, addr + S::A, a.k - kb * kBlockK, kb == lo);
+      mma_stage<BT, false>(tmem, addr, addr + S::A, a.k - kb * kBlockK, kb == lo);
       umma_commit(&pipe.empty[s]);
     }
-    if (it < (uint32_t)(hi - lo)) drain_mmas(drain, a.err);
+    if (it < (uint32_t)(hi - lo)) drain_mmas<false>(drain, a.err);
     else umma_commit(done);
   }
   __syncwarp();
@@ -310,8 +378,7 @@ __global__ void __launch_bounds__(kFewThreads)
   if (warp >= 2) {
     // lane = channel, column = row of x: [row][channel] is written without bank conflicts
     const int q = warp % 4;
-    // the lanes may end a wait that gave up apart
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, a.err, 13));
+    const bool ok = warp_wait(done, 0, a.err, 13);
     tc_after_sync();
     const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
     if (ok) {
@@ -358,7 +425,7 @@ __global__ void __launch_bounds__(kFewThreads)
   if (warp == 1) {
     __syncwarp();
     tc_after_sync();
-    tmem_free(tmem, S::COLS);
+    tmem_free<false>(tmem, S::COLS);
   }
 }
 
@@ -369,11 +436,17 @@ __global__ void __launch_bounds__(kFewThreads)
 constexpr int kGroupRows = 8;  // row tiles per group of the tile order
 
 // Warp 0 issues TMA, warp 1 the MMAs, the others are the epilogue: four, one
-// per quarter of the accumulator's lanes, for every 64 columns.
+// per quarter of the accumulator's lanes, for every 64 columns. Tiles of 256
+// columns are worked on by a pair of CTAs, 128 rows each, which halves what
+// each of them loads of w: with a CTA alone, its shared memory took in 48 KB
+// and gave out as much for every 512 cycles of the tensor core, more than L2
+// delivers (8192^3: 421 us).
 template <int BN>
 struct Tile {
+  static constexpr bool PAIR = BN == 256;
+  static constexpr int ROWS = PAIR ? 256 : 128;
   static constexpr int EPI_WARPS = BN / 16, THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int A = 128 * kBlockK, B = BN * kBlockK, STAGE = A + B;
+  static constexpr int A = 128 * kBlockK, B = BN * kBlockK / (PAIR ? 2 : 1), STAGE = A + B;
   static constexpr int TURN = EPI_WARPS * 4096;       // epilogue warps' outputs on their way
   static constexpr int COLUMN = EPI_WARPS * 64 * 8;   // their channel scales and biases
   static constexpr int STAGES = (227 * 1024 - TURN - COLUMN - 1024 - 256) / STAGE;
@@ -385,11 +458,11 @@ struct Tile {
 // the CTAs at work together share both operands' tiles in L2.
 struct TileOrder {
   uint32_t mtiles, ntiles, total;
-  DMX_DEVICE void at(uint32_t t, int64_t& m0, int& n_tile) const {
+  DMX_DEVICE void at(uint32_t t, uint32_t& m_tile, uint32_t& n_tile) const {
     const uint32_t per = kGroupRows * ntiles, g = t / per, in_group = t - g * per;
     const uint32_t high = min((uint32_t)kGroupRows, mtiles - g * kGroupRows);
-    n_tile = (int)(in_group / high);
-    m0 = (int64_t)(g * kGroupRows + in_group % high) * 128;
+    n_tile = in_group / high;
+    m_tile = g * kGroupRows + in_group % high;
   }
 };
 
@@ -422,6 +495,8 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
                        const __grid_constant__ TileOrder order, int wide) {
   using S = Tile<BN>;
   constexpr int STAGES = S::STAGES;
+  constexpr bool PAIR = S::PAIR;
+  constexpr int kCtas = PAIR ? 2 : 1;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -436,6 +511,8 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = PAIR ? blockIdx.x % 2 : 0;  // in the pair; the first issues its MMAs
+  const uint32_t begin = blockIdx.x / kCtas, step = gridDim.x / kCtas;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&pipe.full[s], 1);
@@ -443,68 +520,74 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 32 * S::EPI_WARPS);
+      mbar_init(&acc_empty[i], kCtas * S::EPI_WARPS);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(slot, S::COLS);
+  if (warp == 1) tmem_alloc<PAIR>(slot, S::COLS);
   tc_before_sync();
-  __syncthreads();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   tc_after_sync();
   const uint32_t tmem = *slot;
   const int blocks = (a.k + kBlockK - 1) / kBlockK;
 
+  // Both warps walk their loops whole, one elected lane issuing: the
+  // descriptors then live in uniform registers, which is where the tensor core
+  // and the copy engine take them from.
+  const bool elected = elect_one();
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (uint32_t t = blockIdx.x; t < order.total && ok; t += gridDim.x) {
-        int64_t m0;
-        int nt;
-        order.at(t, m0, nt);
-        for (int kb = 0; kb < blocks; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 21)) {
-            ok = false;
-            break;
-          }
+    uint32_t it = 0;
+    bool ok = true;
+    for (uint32_t t = begin; t < order.total && ok; t += step) {
+      uint32_t mt, nt;
+      order.at(t, mt, nt);
+      const int m0 = (int)(mt * S::ROWS + rank * 128), n0 = (int)(nt * BN + rank * 128);
+      for (int kb = 0; kb < blocks; ++kb, ++it) {
+        const uint32_t s = it % STAGES;
+        ok = warp_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 21);
+        if (!ok) break;
+        if (elected) {
           unsigned char* dst = smem + s * S::STAGE;
-          mbar_expect_tx(&pipe.full[s], S::STAGE);
-          tma_load_2d(dst, &tm_x, &pipe.full[s], kb * kBlockK, (int)m0);
-          tma_load_2d(dst + S::A, &tm_w, &pipe.full[s], kb * kBlockK, nt * BN);
-        }
-      }
-      if (!ok) drain_loads<STAGES>(pipe, it, a.err);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      int tl = 0;
-      bool ok = true;
-      for (uint32_t t = blockIdx.x; t < order.total && ok; t += gridDim.x, ++tl) {
-        const int acc = tl & 1;
-        if (!mbar_wait(&acc_empty[acc], ((tl >> 1) & 1) ^ 1, a.err, 22)) {
-          ok = false;
-          break;
-        }
-        tc_after_sync();
-        const uint32_t d = tmem + (uint32_t)(acc * BN);
-        for (int kb = 0; kb < blocks; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 23)) {
-            ok = false;
-            break;
+          // a pair's loads count at the first CTA's barrier, where its MMAs wait
+          if (rank == 0) mbar_expect_tx(&pipe.full[s], kCtas * S::STAGE);
+          if (PAIR) {
+            const uint32_t bar = of_rank(&pipe.full[s], 0);
+            tma_load_pair(dst, &tm_x, bar, kb * kBlockK, m0);
+            tma_load_pair(dst + S::A, &tm_w, bar, kb * kBlockK, n0);
+          } else {
+            tma_load_2d(dst, &tm_x, &pipe.full[s], kb * kBlockK, m0);
+            tma_load_2d(dst + S::A, &tm_w, &pipe.full[s], kb * kBlockK, n0);
           }
-          tc_after_sync();
-          const uint32_t addr = smem_u32(smem + s * S::STAGE);
-          mma_stage<BN>(d, addr, addr + S::A, a.k - kb * kBlockK, kb == 0);
-          umma_commit(&pipe.empty[s]);
         }
-        if (ok) umma_commit(&acc_full[acc]);
       }
-      if (!ok) drain_mmas(drain, a.err);
     }
+    if (!ok && rank == 0) drain_loads<STAGES>(pipe, it, a.err);
+  } else if (warp == 1) {
+    uint32_t it = 0;
+    int tl = 0;
+    bool ok = true;
+    for (uint32_t t = begin; t < order.total && ok && rank == 0; t += step, ++tl) {
+      const int acc = tl & 1;
+      ok = warp_wait(&acc_empty[acc], ((tl >> 1) & 1) ^ 1, a.err, 22);
+      if (!ok) break;
+      tc_after_sync();
+      const uint32_t d = tmem + (uint32_t)(acc * BN);
+      for (int kb = 0; kb < blocks; ++kb, ++it) {
+        const uint32_t s = it % STAGES;
+        ok = warp_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 23);
+        if (!ok) break;
+        tc_after_sync();
+        if (elected) {
+          const uint32_t addr = smem_u32(smem + s * S::STAGE);
+          mma_stage<BN, PAIR>(d, addr, addr + S::A, a.k - kb * kBlockK, kb == 0);
+          commit<PAIR>(&pipe.empty[s]);
+        }
+      }
+      if (ok && elected) commit<PAIR>(&acc_full[acc]);
+    }
+    if (!ok && elected) drain_mmas<PAIR>(drain, a.err);
   } else {
     // this warp: rows 32 quarter + lane, columns c_lo .. c_lo + 63 of each tile
     const int quarter = warp % 4, c_lo = (warp - 2) / 4 * 64;
@@ -518,10 +601,13 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
     float4 sb;
     float xs;
     int64_t m0_next;
-    int nt_next;
+    int n0_next;
     auto fetch = [&](uint32_t t) {
-      order.at(t, m0_next, nt_next);
-      const int n = nt_next * BN + c_lo + 2 * lane;
+      uint32_t mt, nt;
+      order.at(t, mt, nt);
+      m0_next = (int64_t)mt * S::ROWS + rank * 128;
+      n0_next = (int)(nt * BN);
+      const int n = n0_next + c_lo + 2 * lane;
       sb = make_float4(1.f, 1.f, 0.f, 0.f);
       if (a.w_scale) {
         if (n < a.n) sb.x = a.w_scale[n];
@@ -536,18 +622,16 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
     };
     bool ok = true;
     int tl = 0;
-    if (blockIdx.x < order.total) fetch(blockIdx.x);
-    for (uint32_t t = blockIdx.x; t < order.total; t += gridDim.x, ++tl) {
+    if (begin < order.total) fetch(begin);
+    for (uint32_t t = begin; t < order.total; t += step, ++tl) {
       const int64_t m0 = m0_next;
-      const int n0 = nt_next * BN, acc = tl & 1;
+      const int n0 = n0_next, acc = tl & 1;
       const float row_scale = xs;
       __syncwarp();
       col[lane] = sb;
       __syncwarp();
-      if (t + gridDim.x < order.total) fetch(t + gridDim.x);
-      if (ok && !mbar_wait(&acc_full[acc], (tl >> 1) & 1, a.err, 24)) ok = false;
-      // the lanes may end a wait that gave up apart
-      ok = __all_sync(0xffffffffu, ok);
+      if (t + step < order.total) fetch(t + step);
+      ok = ok && warp_wait(&acc_full[acc], (tl >> 1) & 1, a.err, 24);
       tc_after_sync();
       if (ok) {
         const int rows = (int)min((int64_t)32, a.rows - m0 - quarter * 32);
@@ -631,16 +715,23 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
         }
       }
       tc_before_sync();
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[acc]))
-                   : "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) arrive_at(of_rank(&acc_empty[acc], 0));
+        else
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[acc]))
+                       : "memory");
+      }
     }
   }
   tc_before_sync();
-  __syncthreads();
+  // a pair's MMAs read both CTAs' memory, and its barriers are the first's
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tc_after_sync();
-    tmem_free(tmem, S::COLS);
+    tmem_free<PAIR>(tmem, S::COLS);
   }
 }
 
@@ -696,21 +787,37 @@ bool launch_few(const LinearArgs& a, cudaStream_t s) {
 
 template <int BN, typename OT, bool GELU>
 bool launch_tile(const LinearArgs& a, cudaStream_t s) {
-  CUtensorMap tw, tx;
-  if (!row_map(&tx, a.x, a.rows, a.k, a.x_ld, 128) || !row_map(&tw, a.w, a.n, a.k, a.w_ld, BN))
-    return false;
   using S = Tile<BN>;
+  constexpr int kCtas = S::PAIR ? 2 : 1;
+  CUtensorMap tw, tx;
+  if (!row_map(&tx, a.x, a.rows, a.k, a.x_ld, 128) ||
+      !row_map(&tw, a.w, a.n, a.k, a.w_ld, BN / kCtas))
+    return false;
   auto kernel = linear_tile_kernel<BN, OT, GELU>;
   static PerDevice once;
   if (once.first()) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
-  const int64_t mtiles = (a.rows + 127) / 128, ntiles = (a.n + BN - 1) / BN;
+  const int64_t mtiles = (a.rows + S::ROWS - 1) / S::ROWS, ntiles = (a.n + BN - 1) / BN;
   if (mtiles * ntiles > INT32_MAX) return false;  // no memory holds such an output
   const TileOrder order = {(uint32_t)mtiles, (uint32_t)ntiles, (uint32_t)(mtiles * ntiles)};
-  const int pitch = sizeof(OT);
-  const bool wide = vec_of(a.out, a.out_ld, pitch) != VEC_NONE &&
-                    (!a.residual || vec_of(a.residual, a.residual_ld, pitch) != VEC_NONE);
-  const unsigned grid = (unsigned)std::min<int64_t>(mtiles * ntiles, sm_count());
-  kernel<<<grid, S::THREADS, S::TOTAL, s>>>(tx, tw, a, order, wide ? 1 : 0);
+  const int bytes = sizeof(OT);
+  const bool wide = vec_of(a.out, a.out_ld, bytes) != VEC_NONE &&
+                    (!a.residual || vec_of(a.residual, a.residual_ld, bytes) != VEC_NONE);
+  const unsigned grid = (unsigned)(kCtas * std::min<int64_t>(mtiles * ntiles, sm_count() / kCtas));
+  if (!S::PAIR) {
+    kernel<<<grid, S::THREADS, S::TOTAL, s>>>(tx, tw, a, order, wide ? 1 : 0);
+    return true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = S::TOTAL;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {kCtas, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, tx, tw, a, order, wide ? 1 : 0);
   return true;
 }
 
@@ -729,14 +836,16 @@ bool launch_typed(const LinearArgs& a, cudaStream_t s) {
     if (a.rows <= 64) return launch_few<64, 4, OT, GELU>(a, s);
     return launch_few<128, 3, OT, GELU>(a, s);
   }
-  // the tile width whose rounds over the SMs take least: a tile costs its
-  // columns and about 32 more for its start and end
-  const int64_t mtiles = (a.rows + 127) / 128, sms = sm_count();
-  auto cost = [&](int bn) {
-    return (mtiles * ((a.n + bn - 1) / bn) + sms - 1) / sms * (bn + 32);
+  // the tile whose rounds over the SMs take least: a tile costs its columns and
+  // about 32 more for its start and end
+  const int64_t sms = sm_count();
+  auto cost = [&](int rows, int bn) {
+    const int64_t tiles = (a.rows + rows - 1) / rows * ((a.n + bn - 1) / bn) * (rows / 128);
+    return (tiles + sms - 1) / sms * (bn + 32);
   };
-  if (cost(256) <= cost(128) && cost(256) <= cost(64)) return launch_tile<256, OT, GELU>(a, s);
-  if (cost(128) <= cost(64)) return launch_tile<128, OT, GELU>(a, s);
+  const int64_t pair = cost(256, 256), half = cost(128, 128), quarter = cost(128, 64);
+  if (pair <= half && pair <= quarter) return launch_tile<256, OT, GELU>(a, s);
+  if (half <= quarter) return launch_tile<128, OT, GELU>(a, s);
   return launch_tile<64, OT, GELU>(a, s);
 }
 
