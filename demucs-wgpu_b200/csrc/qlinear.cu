@@ -231,8 +231,11 @@ DMX_DEVICE uint32_t of_rank(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+// Relaxed: what it announces, reads of tensor memory, is ordered by the
+// tcgen05 fence before it; a release would wait for the thread's stores to
+// global memory (112896x128->2048: 173 us).
 DMX_DEVICE void arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A tile into this CTA's memory, its bytes counted at the first CTA's barrier.
 DMX_DEVICE void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
