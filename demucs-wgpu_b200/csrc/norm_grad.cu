@@ -1,104 +1,98 @@
-// Backward pass of the layer norm (dmx_layer_norm_backward).
-//
-//   h = (x - mean) rstd,  g = dy weight
-//   dx = rstd (g - sum g / C - h sum(g h) / C)
-//   dweight = sum over rows of dy h,  dbias = sum over rows of dy
-//
-// The column sums are taken per block of rows into partial sums, which a
-// second kernel adds in a fixed order: no atomics, so a gradient is the same
-// from call to call.
+// Entry of the layer norm's backward pass (norm_grad.cuh): how many blocks
+// walk the rows, and the join of their column sums.
 #include <algorithm>
 
+#include "dmx.h"
 #include "ops.h"
 #include "ops_common.cuh"
 
 namespace dmx {
 
+#define DMX_GRAD_UNIT(x) void launch_norm_grad_##x(const NormGradArgs& a, int parts, int vec, cudaStream_t s);
+DMX_GRAD_UNIT(f32_f32)
+DMX_GRAD_UNIT(f32_f16)
+DMX_GRAD_UNIT(f32_bf16)
+DMX_GRAD_UNIT(f16_f32)
+DMX_GRAD_UNIT(f16_f16)
+DMX_GRAD_UNIT(f16_bf16)
+DMX_GRAD_UNIT(bf16_f32)
+DMX_GRAD_UNIT(bf16_f16)
+DMX_GRAD_UNIT(bf16_bf16)
+#undef DMX_GRAD_UNIT
+
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxParts = 296;
-
-int64_t parts_of(int64_t rows) { return std::min<int64_t>((rows + 31) / 32, kMaxParts); }
-
-__global__ void __launch_bounds__(kThreads) norm_grad_rows_kernel(const NormGradArgs a) {
-  __shared__ float sh[2][kThreads / 32];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-      const float h = (load_as_f32(a.x, a.x_type, row * a.x_ld + c) - mean) * rstd;
-      float g = load_as_f32(a.dy, a.dy_type, row * a.dy_ld + c);
-      if (a.weight) g *= load_as_f32(a.weight, a.param_type, c);
-      s1 += g;
-      s2 = fmaf(g, h, s2);
-    }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-      sh[0][threadIdx.x >> 5] = s1;
-      sh[1][threadIdx.x >> 5] = s2;
-    }
-    __syncthreads();
-    s1 = s2 = 0.f;
-    for (int i = 0; i < kThreads / 32; ++i) {
-      s1 += sh[0][i];
-      s2 += sh[1][i];
-    }
-    s1 /= (float)a.cols;
-    s2 /= (float)a.cols;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-      const float h = (load_as_f32(a.x, a.x_type, row * a.x_ld + c) - mean) * rstd;
-      float g = load_as_f32(a.dy, a.dy_type, row * a.dy_ld + c);
-      if (a.weight) g *= load_as_f32(a.weight, a.param_type, c);
-      store_from_f32(a.dx, a.x_type, row * a.dx_ld + c, rstd * (g - s1 - h * s2));
-    }
-  }
+// Most blocks that walk the rows: two per SM of a B200; where groups of threads
+// hold a row, one whose rows to come fill the SM's shared memory, or (rows
+// that do not start on 16 bytes) three without. Constants, so that a sum does
+// not depend on the device.
+int64_t most_parts(int64_t cols, bool vec) {
+  return cols <= 1024 || cols > kGradBlockCols ? 296 : vec ? 148 : 444;
 }
 
-// Block (column strip, part): sums of its rows.
-__global__ void __launch_bounds__(kThreads) norm_grad_cols_kernel(const NormGradArgs a, int parts) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.cols) return;
-  float dw = 0.f, db = 0.f;
-  for (int64_t row = blockIdx.y; row < a.rows; row += parts) {
-    const float h = (load_as_f32(a.x, a.x_type, row * a.x_ld + c) - a.mean[row]) * a.rstd[row];
-    const float d = load_as_f32(a.dy, a.dy_type, row * a.dy_ld + c);
-    dw = fmaf(d, h, dw);
-    db += d;
-  }
-  a.partials[((int64_t)blockIdx.y * 2) * a.cols + c] = dw;
-  a.partials[((int64_t)blockIdx.y * 2 + 1) * a.cols + c] = db;
+// As many of them as give each the same number of turns.
+int parts_of(int64_t rows, int64_t cols, bool vec) {
+  const int64_t each = cols <= 128 ? 32 : cols <= 256 ? 16 : cols <= 1024 ? 8
+                       : cols <= kGradBlockCols ? grad_groups((int)cols) : 1;
+  const int64_t most = most_parts(cols, vec);
+  const int64_t units = (rows + each - 1) / each, turns = (units + most - 1) / most;
+  return turns ? (int)((units + turns - 1) / turns) : 0;
 }
 
-__global__ void __launch_bounds__(kThreads) norm_grad_join_kernel(const NormGradArgs a, int parts) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.cols) return;
-  float dw = 0.f, db = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    dw += a.partials[((int64_t)p * 2) * a.cols + c];
-    db += a.partials[((int64_t)p * 2 + 1) * a.cols + c];
-  }
-  if (a.dweight) a.dweight[c] = dw;
-  if (a.dbias) a.dbias[c] = db;
+// 32 columns per block; each of its 32 warps adds a share of the parts, whose
+// sums are joined in order.
+__global__ void __launch_bounds__(1024)
+    norm_grad_join_kernel(const float* __restrict__ partials, int parts, int cols,
+                          float* __restrict__ dweight, float* __restrict__ dbias) {
+  __shared__ float sh[2][32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float w = 0.f, b = 0.f;
+  if (c < cols)
+#pragma unroll 5
+    for (int p = warp; p < parts; p += 32) {
+      w += partials[(int64_t)(2 * p) * cols + c];
+      b += partials[(int64_t)(2 * p + 1) * cols + c];
+    }
+  sh[0][warp][lane] = w;
+  sh[1][warp][lane] = b;
+  __syncthreads();
+  const int mine = blockIdx.x * 32 + warp;  // this warp's column
+  w = warp_sum(sh[0][lane][warp]);
+  b = warp_sum(sh[1][lane][warp]);
+  if (lane != 0 || mine >= cols) return;
+  if (dweight) dweight[mine] = w;
+  if (dbias) dbias[mine] = b;
 }
 
 }  // namespace
 
 size_t norm_grad_workspace(int64_t rows, int64_t cols) {
-  return (size_t)parts_of(rows) * 2 * (size_t)cols * sizeof(float);
+  const int parts = std::max(parts_of(rows, cols, true), parts_of(rows, cols, false));
+  return (size_t)parts * 2 * (size_t)cols * sizeof(float);
 }
 
-void launch_norm_grad(const NormGradArgs& a, cudaStream_t s) {
-  const int parts = (int)parts_of(a.rows);
-  const unsigned strips = (unsigned)((a.cols + kThreads - 1) / kThreads);
-  if (a.dweight || a.dbias) {  // first: dx may be written over x or dy
-    if (parts > 0) norm_grad_cols_kernel<<<dim3(strips, parts), kThreads, 0, s>>>(a, parts);
-    norm_grad_join_kernel<<<strips, kThreads, 0, s>>>(a, parts);
+void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
+  NormGradArgs a = args;
+  const bool sums = a.dweight || a.dbias;
+  if (!sums) a.partials = nullptr;
+  int vec = std::min(vec_of(a.x, a.x_ld, type_size(a.x_type)), vec_of(a.dy, a.dy_ld, type_size(a.dy_type)));
+  vec = std::min(vec, vec_of(a.weight, 0, type_size(a.param_type)));
+  if (a.dx) vec = std::min(vec, vec_of(a.dx, a.dx_ld, type_size(a.x_type)));
+  // the long rows' partial sums are stored by pieces too
+  if (a.partials && a.cols > kGradBlockCols) vec = std::min(vec, vec_of(a.partials, a.cols, 4));
+  const int parts = parts_of(a.rows, a.cols, vec != VEC_NONE);
+  if (parts > 0 && (sums || a.dx)) {
+    using Launch = void (*)(const NormGradArgs&, int, int, cudaStream_t);
+    // by dmx_type of x and of dy: F32, F16, BF16
+    static const Launch launch[3][3] = {
+        {launch_norm_grad_f32_f32, launch_norm_grad_f32_f16, launch_norm_grad_f32_bf16},
+        {launch_norm_grad_f16_f32, launch_norm_grad_f16_f16, launch_norm_grad_f16_bf16},
+        {launch_norm_grad_bf16_f32, launch_norm_grad_bf16_f16, launch_norm_grad_bf16_bf16}};
+    launch[a.x_type][a.dy_type](a, parts, vec, s);
   }
-  if (a.dx && a.rows > 0)
-    norm_grad_rows_kernel<<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), kThreads, 0, s>>>(a);
+  if (sums)
+    norm_grad_join_kernel<<<(a.cols + 31) / 32, 1024, 0, s>>>(a.partials, parts, a.cols, a.dweight,
+                                                             a.dbias);
 }
 
 }  // namespace dmx

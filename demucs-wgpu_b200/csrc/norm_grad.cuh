@@ -1,0 +1,439 @@
+// Backward pass of the layer norm (dmx_layer_norm_backward).
+//
+//   h = (x - mean) rstd,  g = dy weight
+//   dx = rstd (g - sum g / C - h sum(g h) / C)
+//   dweight = sum over rows of dy h,  dbias = sum over rows of dy
+//
+// Bound by HBM: x and dy are read once and dx written once. A block walks rows
+// a grid apart; each thread keeps the same columns in every row, so the column
+// sums stay with it (in registers, or in shared memory for long rows) and
+// leave once, as one partial sum per block and column. A second kernel adds
+// the blocks' sums in a fixed order: no atomics, a gradient is the same from
+// call to call. Rows of up to 1024 columns belong to a warp (or half or a
+// quarter of one); longer ones to a group of up to 1024 threads, which copies
+// the rows to come into shared memory while it works on one (each thread what
+// it will read itself, so nothing waits on the others for that). Rows longer
+// than that are swept twice, for dx and for the column sums, re-read from L2.
+#pragma once
+
+#include <algorithm>
+
+#include "ops.h"
+#include "ops_common.cuh"
+
+namespace dmx {
+
+// Values of piece j of dy, x and the weight to g = dy w and h.
+template <typename XT, typename DT, typename PT, bool VEC>
+struct GradPiece {
+  float d[8], h[8], g[8];
+  DMX_DEVICE void unpack(const uint32_t* draw, const uint32_t* xraw, const uint32_t* wraw, bool weight,
+                         float mean, float rstd) {
+    Pieces<VEC>::template unpack<DT>(draw, d);
+    Pieces<VEC>::template unpack<XT>(xraw, h);
+    centre8(h, mean);
+    scale8(h, rstd);
+    if (weight) {
+      Pieces<VEC>::template unpack<PT>(wraw, g);
+      times8(g, d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = d[e];
+    }
+  }
+};
+
+DMX_DEVICE float2 dot_sums(const float* g, const float* h, float2 s) {
+  // (sum g, sum g h) over eight values
+  float2 a = make_float2(0.f, 0.f), b = a;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 g2 = make_float2(g[e], g[e + 1]);
+    a = __fadd2_rn(a, g2);
+    b = __ffma2_rn(g2, make_float2(h[e], h[e + 1]), b);
+  }
+  return make_float2(s.x + (a.x + a.y), s.y + (b.x + b.y));
+}
+// v = rstd (g - m1 - h m2)
+DMX_DEVICE void dx8(const float* g, const float* h, float m1, float m2, float rstd, float* v) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 h2 = make_float2(h[e], h[e + 1]);
+    float2 t = __fadd2_rn(make_float2(g[e], g[e + 1]), make_float2(-m1, -m1));
+    t = __ffma2_rn(h2, make_float2(-m2, -m2), t);
+    t = __fmul2_rn(t, make_float2(rstd, rstd));
+    v[e] = t.x;
+    v[e + 1] = t.y;
+  }
+}
+DMX_DEVICE void gather8(float* w, float* b, const float* d, const float* h) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 d2 = make_float2(d[e], d[e + 1]);
+    const float2 r = __ffma2_rn(d2, make_float2(h[e], h[e + 1]), make_float2(w[e], w[e + 1]));
+    const float2 s = __fadd2_rn(make_float2(b[e], b[e + 1]), d2);
+    w[e] = r.x;
+    w[e + 1] = r.y;
+    b[e] = s.x;
+    b[e + 1] = s.y;
+  }
+}
+
+// Sums of (a, b) over the threads of one row.
+template <int LANES>
+DMX_DEVICE float2 lanes_sum2(float2 v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  return v;
+}
+
+constexpr int kGradThreads = 256;
+
+// Rows of up to LANES * NV * 8 columns, LANES lanes each.
+template <typename XT, typename DT, typename PT, int LANES, int NV, bool VEC>
+__global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
+    norm_grad_warp_kernel(const __grid_constant__ NormGradArgs a, bool wide) {
+  constexpr int per = kGradThreads / LANES, kCols = LANES * NV * 8;
+  __shared__ float sums[per][kCols];
+  const Pieces<VEC> p = {(int)(threadIdx.x % LANES), LANES, a.cols, wide};
+  const XT* x = static_cast<const XT*>(a.x);
+  const DT* dy = static_cast<const DT*>(a.dy);
+  const PT* weight = static_cast<const PT*>(a.weight);
+  uint32_t wraw[NV][8], xraw[NV][8], draw[NV][8];
+  float dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (weight) p.fetch(weight, j, wraw[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[j][e] = db[j][e] = 0.f;
+  }
+  const int64_t step = (int64_t)gridDim.x * per;
+  int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / LANES;
+  float mean = 0.f, rstd = 0.f;
+  // a row past the last one is zeros: it adds nothing and only takes part in the shuffles
+  auto fetch = [&](int64_t r) {
+    const bool live = r < a.rows;
+    const Pieces<VEC> q = {p.t, LANES, live ? a.cols : 0, wide};
+    const int64_t at = live ? r : 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      q.fetch(x + at * a.x_ld, j, xraw[j]);
+      q.fetch(dy + at * a.dy_ld, j, draw[j]);
+    }
+    mean = live ? a.mean[at] : 0.f;
+    rstd = live ? a.rstd[at] : 0.f;
+  };
+  const int64_t passes = (a.rows + step - 1) / step;
+  for (int64_t pass = 0; pass < passes; ++pass, row += step) {
+    fetch(row);
+    GradPiece<XT, DT, PT, VEC> q[NV];
+    float2 s = make_float2(0.f, 0.f);
+    const float row_mean = mean, row_rstd = rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      q[j].unpack(draw[j], xraw[j], wraw[j], weight != nullptr, row_mean, row_rstd);
+      s = dot_sums(q[j].g, q[j].h, s);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) gather8(dw[j], db[j], q[j].d, q[j].h);
+    if (!a.dx) continue;
+    s = lanes_sum2<LANES>(s);
+    if (row >= a.rows) continue;
+    const float m1 = s.x / (float)a.cols, m2 = s.y / (float)a.cols;
+    XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float v[8];
+      dx8(q[j].g, q[j].h, m1, m2, row_rstd, v);
+      p.store(dx, j, v);
+    }
+  }
+  if (!a.partials) return;
+  // the block's row groups added in their order
+  float* out = a.partials + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        sums[threadIdx.x / LANES][p.col(j, e)] = half ? db[j][e] : dw[j][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cols; c += kGradThreads) {
+      float t = 0.f;
+#pragma unroll
+      for (int g = 0; g < per; ++g) t += sums[g][c];
+      out[half * a.cols + c] = t;
+    }
+  }
+}
+
+// `bytes` (0..16, the rest as zeros) of 16 from global to this thread's shared memory.
+DMX_DEVICE void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
+}
+
+// Rows of up to blockDim.x * 16 columns, a group of blockDim.x threads each;
+// blockDim.y groups to a block. Shared memory, all of it each thread's own and
+// laid out with the thread innermost: the column sums, (dw, db) of two columns
+// to 16 bytes, and with VEC the `ahead` rows to come.
+template <typename XT, typename DT, typename PT, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+    norm_grad_block_kernel(const __grid_constant__ NormGradArgs a, bool wide, int ahead) {
+  constexpr int NV = 2, kXUnits = sizeof(XT) / 2, kDUnits = sizeof(DT) / 2;  // of 16 bytes per piece
+  constexpr int kStage = NV * (kXUnits + kDUnits);
+  extern __shared__ float4 own[];
+  __shared__ float2 sh[2][32];
+  const int n = blockDim.x * blockDim.y, id = threadIdx.y * blockDim.x + threadIdx.x;
+  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
+  const XT* x = static_cast<const XT*>(a.x);
+  const DT* dy = static_cast<const DT*>(a.dy);
+  const PT* weight = static_cast<const PT*>(a.weight);
+  const int lane = id & 31, warp = id >> 5, warps = blockDim.x / 32;
+#pragma unroll
+  for (int i = 0; i < NV * 4; ++i) own[i * n + id] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* ring = own + NV * 4 * n + id;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  // the copies of one row into stage s of the ring; an empty group past the end
+  auto copy_row = [&](int64_t row, int s) {
+    if (row < a.rows) {
+      const uint32_t at = ring_at + (uint32_t)(s * kStage * n) * 16;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = p.col(j, 0);
+        const XT* xs = x + row * a.x_ld;
+        const DT* ds = dy + row * a.dy_ld;
+#pragma unroll
+        for (int u = 0; u < kXUnits; ++u) {
+          const int from = c + u * (16 / (int)sizeof(XT));
+          const int bytes = min(max((a.cols - from) * (int)sizeof(XT), 0), 16);
+          copy16(at + (uint32_t)((j * kXUnits + u) * n) * 16, xs + (bytes ? from : 0), bytes);
+        }
+#pragma unroll
+        for (int u = 0; u < kDUnits; ++u) {
+          const int from = c + u * (16 / (int)sizeof(DT));
+          const int bytes = min(max((a.cols - from) * (int)sizeof(DT), 0), 16);
+          copy16(at + (uint32_t)((NV * kXUnits + j * kDUnits + u) * n) * 16, ds + (bytes ? from : 0),
+                 bytes);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (VEC)
+    for (int s = 0; s < ahead; ++s) copy_row(first + s * step, s);
+  uint32_t wraw[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (weight) p.fetch(weight, j, wraw[j]);
+  int turn = 0, stage = 0;
+  for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    uint32_t xraw[NV][8], draw[NV][8];
+    if (VEC) {
+      // every row's copies are a group: the oldest of `ahead` has landed
+      if (ahead == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else if (ahead == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else asm volatile("cp.async.wait_group 3;" ::: "memory");
+      const float4* from = ring + stage * kStage * n;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int u = 0; u < kXUnits; ++u)
+          *reinterpret_cast<float4*>(&xraw[j][4 * u]) = from[(j * kXUnits + u) * n];
+#pragma unroll
+        for (int u = 0; u < kDUnits; ++u)
+          *reinterpret_cast<float4*>(&draw[j][4 * u]) = from[(NV * kXUnits + j * kDUnits + u) * n];
+      }
+      copy_row(row + ahead * step, stage);
+      stage = stage + 1 == ahead ? 0 : stage + 1;
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        p.fetch(x + row * a.x_ld, j, xraw[j]);
+        p.fetch(dy + row * a.dy_ld, j, draw[j]);
+      }
+    }
+    float2 s = make_float2(0.f, 0.f);
+    GradPiece<XT, DT, PT, VEC> q;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      q.unpack(draw[j], xraw[j], wraw[j], weight != nullptr, mean, rstd);
+      s = dot_sums(q.g, q.h, s);
+      if (a.partials)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float4* o = &own[(j * 4 + i) * n + id];
+          float4 t = *o;
+          t.x = fmaf(q.d[2 * i], q.h[2 * i], t.x);
+          t.y += q.d[2 * i];
+          t.z = fmaf(q.d[2 * i + 1], q.h[2 * i + 1], t.z);
+          t.w += q.d[2 * i + 1];
+          *o = t;
+        }
+    }
+    if (!a.dx) continue;
+    s = lanes_sum2<32>(s);
+    // two buffers in turn: the last row's may still be read
+    if (lane == 0) sh[turn][warp] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
+    s = lanes_sum2<32>(lane < warps ? sh[turn][threadIdx.y * warps + lane] : make_float2(0.f, 0.f));
+    const float m1 = s.x / (float)a.cols, m2 = s.y / (float)a.cols;
+    XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float v[8];
+      q.unpack(draw[j], xraw[j], wraw[j], weight != nullptr, mean, rstd);
+      dx8(q.g, q.h, m1, m2, rstd, v);
+      p.store(dx, j, v);
+    }
+  }
+  if (!a.partials) return;
+  __syncthreads();
+  if (threadIdx.y != 0) return;
+  // the block's groups added in their order
+  float* out = a.partials + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float4 t = own[(j * 4 + i) * n + id];
+      for (int g = 1; g < (int)blockDim.y; ++g) {
+        const float4 u = own[(j * 4 + i) * n + g * blockDim.x + threadIdx.x];
+        t = make_float4(t.x + u.x, t.y + u.y, t.z + u.z, t.w + u.w);
+      }
+      if (p.has(j, 2 * i)) {
+        out[p.col(j, 2 * i)] = t.x;
+        out[a.cols + p.col(j, 2 * i)] = t.y;
+      }
+      if (p.has(j, 2 * i + 1)) {
+        out[p.col(j, 2 * i + 1)] = t.z;
+        out[a.cols + p.col(j, 2 * i + 1)] = t.w;
+      }
+    }
+}
+
+// Rows too long for a block's registers: dx, re-reading the row.
+template <typename XT, typename DT, typename PT, bool VEC>
+__global__ void __launch_bounds__(1024)
+    norm_grad_long_kernel(const __grid_constant__ NormGradArgs a, bool wide) {
+  __shared__ float2 sh[2][32];
+  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
+  const int pieces = (a.cols - 1) / ((int)blockDim.x * 8) + 1;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
+    const DT* dy = static_cast<const DT*>(a.dy) + row * a.dy_ld;
+    XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    GradPiece<XT, DT, PT, VEC> q;
+    auto piece = [&](int j) {
+      uint32_t xraw[8], draw[8], wraw[8];
+      p.fetch(x, j, xraw);
+      p.fetch(dy, j, draw);
+      if (a.weight) p.fetch(static_cast<const PT*>(a.weight), j, wraw);
+      q.unpack(draw, xraw, wraw, a.weight != nullptr, mean, rstd);
+    };
+    float2 s = make_float2(0.f, 0.f);
+    for (int j = 0; j < pieces; ++j) {
+      piece(j);
+      s = dot_sums(q.g, q.h, s);
+    }
+    s = lanes_sum2<32>(s);
+    if (lane == 0) sh[turn][warp] = s;
+    __syncthreads();
+    s = lanes_sum2<32>(lane < warps ? sh[turn][lane] : make_float2(0.f, 0.f));
+    const float m1 = s.x / (float)a.cols, m2 = s.y / (float)a.cols;
+    for (int j = 0; j < pieces; ++j) {
+      piece(j);
+      float v[8];
+      dx8(q.g, q.h, m1, m2, rstd, v);
+      p.store(dx, j, v);
+    }
+  }
+}
+
+// The column sums of such rows: block (strip of 8 columns per thread, part).
+template <typename XT, typename DT, bool VEC>
+__global__ void __launch_bounds__(kGradThreads)
+    norm_grad_columns_kernel(const __grid_constant__ NormGradArgs a, bool wide) {
+  const int pieces = (a.cols - 1) / (kGradThreads * 8) + 1, j = blockIdx.x;
+  const Pieces<VEC> p = {(int)threadIdx.x, kGradThreads, a.cols, wide};
+  if (j >= pieces || !p.has(j, 0)) return;
+  float dw[8] = {}, db[8] = {};
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float d[8], h[8];
+    p.load(static_cast<const XT*>(a.x) + row * a.x_ld, j, h);
+    p.load(static_cast<const DT*>(a.dy) + row * a.dy_ld, j, d);
+    centre8(h, a.mean[row]);
+    scale8(h, a.rstd[row]);
+    gather8(dw, db, d, h);
+  }
+  float* out = a.partials + (int64_t)blockIdx.y * 2 * a.cols;
+  p.store(out, j, dw);
+  p.store(out + a.cols, j, db);
+}
+
+template <typename XT, typename DT, typename PT, bool VEC, int THREADS>
+void launch_norm_grad_block(const NormGradArgs& a, int parts, dim3 block, size_t smem, bool wide,
+                            int ahead, cudaStream_t s) {
+  auto kernel = norm_grad_block_kernel<XT, DT, PT, VEC, THREADS>;
+  static PerDevice once;
+  if (once.first())
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  kernel<<<parts, block, smem, s>>>(a, wide, ahead);
+}
+
+// What norm_grad.cu decides: parts (blocks whose partial sums are joined).
+template <typename XT, typename DT, typename PT, bool VEC>
+void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStream_t s) {
+  if (a.cols <= 64)
+    norm_grad_warp_kernel<XT, DT, PT, 8, 1, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+  else if (a.cols <= 128)
+    norm_grad_warp_kernel<XT, DT, PT, 8, 2, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+  else if (a.cols <= 256)
+    norm_grad_warp_kernel<XT, DT, PT, 16, 2, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+  else if (a.cols <= 512)
+    norm_grad_warp_kernel<XT, DT, PT, 32, 2, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+  else if (a.cols <= 1024)
+    norm_grad_warp_kernel<XT, DT, PT, 32, 4, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+  else if (a.cols <= kGradBlockCols) {
+    const int threads = grad_group_threads(a.cols), groups = grad_groups(a.cols);
+    // shared memory per thread: its sums, and the rows to come
+    const int own = 128, stage = 16 * (sizeof(XT) + sizeof(DT));
+    const int most = 220 * 1024 / (threads * groups);
+    const int ahead = VEC ? std::min(4, (most - own) / stage) : 0;
+    const dim3 block(threads, groups);
+    const size_t smem = (size_t)threads * groups * (own + ahead * stage);
+    if (VEC && ahead < 1)
+      launch_norm_grad_block<XT, DT, PT, false, 1024>(a, parts, block, smem, wide, ahead, s);
+    else if (threads * groups <= 512)
+      launch_norm_grad_block<XT, DT, PT, VEC, 512>(a, parts, block, smem, wide, ahead, s);
+    else
+      launch_norm_grad_block<XT, DT, PT, VEC, 1024>(a, parts, block, smem, wide, ahead, s);
+  } else {
+    const unsigned strips = (unsigned)((a.cols - 1) / (kGradThreads * 8) + 1);
+    // first: dx may be written over x or dy
+    if (a.partials)
+      norm_grad_columns_kernel<XT, DT, VEC><<<dim3(strips, parts), kGradThreads, 0, s>>>(a, wide);
+    if (a.dx)
+      norm_grad_long_kernel<XT, DT, PT, VEC>
+          <<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a, wide);
+  }
+}
+
+template <typename XT, typename DT, typename PT>
+void launch_norm_grad_typed(const NormGradArgs& a, int parts, int vec, cudaStream_t s) {
+  if (vec == VEC_NONE) launch_norm_grad_vec<XT, DT, PT, false>(a, parts, false, s);
+  else launch_norm_grad_vec<XT, DT, PT, true>(a, parts, vec == VEC_32, s);
+}
+
+}  // namespace dmx

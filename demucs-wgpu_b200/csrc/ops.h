@@ -55,6 +55,13 @@ struct NormGradArgs {
   float* dbias = nullptr;    // may be null
   float* partials = nullptr;
 };
+constexpr int kGradBlockCols = 16384;  // longest row that a group of threads holds
+// Threads of such a group (16 columns each), and groups in a block of about 512.
+inline int grad_group_threads(int cols) { return (cols + 511) / 512 * 32; }
+inline int grad_groups(int cols) {
+  const int threads = grad_group_threads(cols);
+  return threads >= 512 ? 1 : 512 / threads;
+}
 size_t norm_grad_workspace(int64_t rows, int64_t cols);
 void launch_norm_grad(const NormGradArgs& a, cudaStream_t s);
 

@@ -231,9 +231,17 @@ DMX_DEVICE uint32_t of_rank(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+DMX_DEVICE int4 ld_cluster(uint32_t at) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
 // Relaxed: what it announces, reads of tensor memory, is ordered by the
 // tcgen05 fence before it; a release would wait for the thread's stores to
-// global memory (112896x128->2048: 173 us).
+// global memory (112896x128->2048: 173 us against 131).
 DMX_DEVICE void arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -319,7 +327,8 @@ struct FewSmem {
 template <int BT, int STAGES, typename OT, bool GELU>
 __global__ void __launch_bounds__(kFewThreads)
     linear_few_kernel(const __grid_constant__ CUtensorMap tm_w,
-                      const __grid_constant__ CUtensorMap tm_x, const LinearArgs a, int splits) {
+                      const __grid_constant__ CUtensorMap tm_x,
+                      const __grid_constant__ LinearArgs a, int splits, int wide) {
   using S = FewSmem<BT, STAGES>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -352,29 +361,37 @@ __global__ void __launch_bounds__(kFewThreads)
   tc_after_sync();
   const uint32_t tmem = *slot;
 
-  if (warp == 0 && lane == 0) {
+  const bool elected = elect_one();
+  const uint32_t count = (uint32_t)(hi - lo);
+  if (warp == 0) {
     uint32_t it = 0;
     for (int kb = lo; kb < hi; ++kb, ++it) {
-      const int s = it % STAGES;
-      if (!mbar_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 11)) break;
-      unsigned char* dst = smem + s * S::STAGE;
-      mbar_expect_tx(&pipe.full[s], S::STAGE);
-      tma_load_2d(dst, &tm_w, &pipe.full[s], kb * kBlockK, n0);
-      tma_load_2d(dst + S::A, &tm_x, &pipe.full[s], kb * kBlockK, m0);
+      const uint32_t s = it % STAGES;
+      if (!warp_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 11)) break;
+      if (elected) {
+        unsigned char* dst = smem + s * S::STAGE;
+        mbar_expect_tx(&pipe.full[s], S::STAGE);
+        tma_load_2d(dst, &tm_w, &pipe.full[s], kb * kBlockK, n0);
+        tma_load_2d(dst + S::A, &tm_x, &pipe.full[s], kb * kBlockK, m0);
+      }
     }
-    if (it < (uint32_t)(hi - lo)) drain_loads<STAGES>(pipe, it, a.err);
-  } else if (warp == 1 && lane == 0) {
+    if (it < count) drain_loads<STAGES>(pipe, it, a.err);
+  } else if (warp == 1) {
     uint32_t it = 0;
     for (int kb = lo; kb < hi; ++kb, ++it) {
-      const int s = it % STAGES;
-      if (!mbar_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 12)) break;
+      const uint32_t s = it % STAGES;
+      if (!warp_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 12)) break;
       tc_after_sync();
-      const uint32_t addr = smem_u32(smem + s * S::STAGE);
-      mma_stage<BT, false>(tmem, addr, addr + S::A, a.k - kb * kBlockK, kb == lo);
-      umma_commit(&pipe.empty[s]);
+      if (elected) {
+        const uint32_t addr = smem_u32(smem + s * S::STAGE);
+        mma_stage<BT, false>(tmem, addr, addr + S::A, a.k - kb * kBlockK, kb == lo);
+        umma_commit(&pipe.empty[s]);
+      }
     }
-    if (it < (uint32_t)(hi - lo)) drain_mmas<false>(drain, a.err);
-    else umma_commit(done);
+    if (elected) {
+      if (it < count) drain_mmas<false>(drain, a.err);
+      else umma_commit(done);
+    }
   }
   __syncwarp();
   int* part = reinterpret_cast<int*>(smem);  // [BT][128]
@@ -398,29 +415,50 @@ __global__ void __launch_bounds__(kFewThreads)
   }
   if (splits > 1) cluster_sync();
   else __syncthreads();
-  // each CTA of the cluster finishes its share of the rows
-  const int rows = (int)min((int64_t)BT, a.rows - m0), cols = min(128, a.n - n0);
-  for (int i = threadIdx.x; i < rows * 128; i += kFewThreads) {
-    const int m = i / 128, c = i % 128;
-    if (m % splits != split || c >= cols) continue;
-    int acc = 0;
-    if (splits > 1) {
-      const uint32_t at = smem_u32(part + m * 128 + c);
-      for (int p = 0; p < splits; ++p) {
-        uint32_t peer;
-        int v;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(p));
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(peer) : "memory");
-        acc += v;
-      }
-    } else {
-      acc = part[m * 128 + c];
+  // each CTA of the cluster finishes its share of the rows, a warp a row and a
+  // lane four channels of it
+  const int rows = (int)min((int64_t)BT, a.rows - m0), n = n0 + 4 * lane;
+  if (n < a.n) {
+    float ws[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ws[i] = n + i < a.n && a.w_scale ? a.w_scale[n + i] : 1.f;
+      b[i] = n + i < a.n && a.bias ? a.bias[n + i] : 0.f;
     }
-    const int n = n0 + c;
-    const int64_t row = m0 + m;
-    store_out<OT>(a, row, n,
-                  linear_value<GELU>(acc, a.x_scale ? a.x_scale[row] : 1.f,
-                                         a.w_scale ? a.w_scale[n] : 1.f, a.bias ? a.bias[n] : 0.f));
+    for (int m = split + warp * splits; m < rows; m += kFewThreads / 32 * splits) {
+      const int4* at = reinterpret_cast<const int4*>(part + m * 128) + lane;
+      int4 acc = make_int4(0, 0, 0, 0);
+      if (splits > 1) {
+        int4 v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p < splits) v[p] = ld_cluster(of_rank(at, p));
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p < splits)
+            acc = make_int4(acc.x + v[p].x, acc.y + v[p].y, acc.z + v[p].z, acc.w + v[p].w);
+      } else {
+        acc = *at;
+      }
+      const int64_t row = m0 + m;
+      const float xs = a.x_scale ? a.x_scale[row] : 1.f;
+      float2 y[2] = {scaled2(acc.x, acc.y, xs, make_float2(ws[0], ws[1]), make_float2(b[0], b[1])),
+                     scaled2(acc.z, acc.w, xs, make_float2(ws[2], ws[3]), make_float2(b[2], b[3]))};
+      if (GELU) gelu_pairs<2>(y);
+      if (wide && n + 4 <= a.n) {
+        float4 f = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+        if (a.residual) {
+          const float4 r = load4(static_cast<const OT*>(a.residual) + row * a.residual_ld + n);
+          f = make_float4(f.x + r.x, f.y + r.y, f.z + r.z, f.w + r.w);
+        }
+        store4(static_cast<OT*>(a.out) + row * a.out_ld + n, f);
+      } else {
+        const float f[4] = {y[0].x, y[0].y, y[1].x, y[1].y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < a.n) store_out<OT>(a, row, n + i, f[i]);
+      }
+    }
   }
   // a peer may still be reading this CTA's partial sums
   if (splits > 1) cluster_sync();
@@ -760,6 +798,14 @@ void launch_gemv(const LinearArgs& a, cudaStream_t s) {
   linear_gemv_kernel<M, C, OT, GELU><<<(a.n + per - 1) / per, kGemvThreads, 0, s>>>(a, kw);
 }
 
+// Whether the rows of out and residual start on 16 bytes.
+template <typename OT>
+int wide_rows(const LinearArgs& a) {
+  const int bytes = sizeof(OT);
+  return vec_of(a.out, a.out_ld, bytes) != VEC_NONE &&
+         (!a.residual || vec_of(a.residual, a.residual_ld, bytes) != VEC_NONE);
+}
+
 template <int BT, int STAGES, typename OT, bool GELU>
 bool launch_few(const LinearArgs& a, cudaStream_t s) {
   CUtensorMap tw, tx;
@@ -784,7 +830,7 @@ bool launch_few(const LinearArgs& a, cudaStream_t s) {
   attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, tw, tx, a, splits);
+  cudaLaunchKernelEx(&cfg, kernel, tw, tx, a, splits, wide_rows<OT>(a));
   return true;
 }
 
@@ -802,12 +848,10 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
   const int64_t mtiles = (a.rows + S::ROWS - 1) / S::ROWS, ntiles = (a.n + BN - 1) / BN;
   if (mtiles * ntiles > INT32_MAX) return false;  // no memory holds such an output
   const TileOrder order = {(uint32_t)mtiles, (uint32_t)ntiles, (uint32_t)(mtiles * ntiles)};
-  const int bytes = sizeof(OT);
-  const bool wide = vec_of(a.out, a.out_ld, bytes) != VEC_NONE &&
-                    (!a.residual || vec_of(a.residual, a.residual_ld, bytes) != VEC_NONE);
+  const int wide = wide_rows<OT>(a);
   const unsigned grid = (unsigned)(kCtas * std::min<int64_t>(mtiles * ntiles, sm_count() / kCtas));
   if (!S::PAIR) {
-    kernel<<<grid, S::THREADS, S::TOTAL, s>>>(tx, tw, a, order, wide ? 1 : 0);
+    kernel<<<grid, S::THREADS, S::TOTAL, s>>>(tx, tw, a, order, wide);
     return true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -820,7 +864,7 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
   attr[0].val.clusterDim = {kCtas, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, tx, tw, a, order, wide ? 1 : 0);
+  cudaLaunchKernelEx(&cfg, kernel, tx, tw, a, order, wide);
   return true;
 }
 
