@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
   const Pieces<VEC> p = {(int)(threadIdx.x % LANES), LANES, a.cols, wide};
   const XT* x = static_cast<const XT*>(a.x);
   const DT* dy = static_cast<const DT*>(a.dy);
-  const PT* weight = static_cast<const PT*>(a.weight);
+  const auto weight = array_of(a.weight, a.param_type, PT());
   uint32_t wraw[NV][8], xraw[NV][8], draw[NV][8];
   float dw[NV][8], db[NV][8];
 #pragma unroll
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
     const float row_mean = mean, row_rstd = rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      q[j].unpack(draw[j], xraw[j], wraw[j], weight != nullptr, row_mean, row_rstd);
+      q[j].unpack(draw[j], xraw[j], wraw[j], a.weight != nullptr, row_mean, row_rstd);
       s = dot_sums(q[j].g, q[j].h, s);
     }
 #pragma unroll
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(THREADS)
   const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   const XT* x = static_cast<const XT*>(a.x);
   const DT* dy = static_cast<const DT*>(a.dy);
-  const PT* weight = static_cast<const PT*>(a.weight);
+  const auto weight = array_of(a.weight, a.param_type, PT());
   const int lane = id & 31, warp = id >> 5, warps = blockDim.x / 32;
 #pragma unroll
   for (int i = 0; i < NV * 4; ++i) own[i * n + id] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(THREADS)
     GradPiece<XT, DT, PT, VEC> q;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      q.unpack(draw[j], xraw[j], wraw[j], weight != nullptr, mean, rstd);
+      q.unpack(draw[j], xraw[j], wraw[j], a.weight != nullptr, mean, rstd);
       s = dot_sums(q.g, q.h, s);
       if (a.partials)
 #pragma unroll
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float v[8];
-      q.unpack(draw[j], xraw[j], wraw[j], weight != nullptr, mean, rstd);
+      q.unpack(draw[j], xraw[j], wraw[j], a.weight != nullptr, mean, rstd);
       dx8(q.g, q.h, m1, m2, rstd, v);
       p.store(dx, j, v);
     }
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(1024)
       uint32_t xraw[8], draw[8], wraw[8];
       p.fetch(x, j, xraw);
       p.fetch(dy, j, draw);
-      if (a.weight) p.fetch(static_cast<const PT*>(a.weight), j, wraw);
+      if (a.weight) p.fetch(array_of(a.weight, a.param_type, PT()), j, wraw);
       q.unpack(draw, xraw, wraw, a.weight != nullptr, mean, rstd);
     };
     float2 s = make_float2(0.f, 0.f);
@@ -413,8 +413,8 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const int ahead = VEC ? std::min(4, (most - own) / stage) : 0;
     const dim3 block(threads, groups);
     const size_t smem = (size_t)threads * groups * (own + ahead * stage);
-    if (VEC && ahead < 1)
-      launch_norm_grad_block<XT, DT, PT, false, 1024>(a, parts, block, smem, wide, ahead, s);
+    if (VEC && ahead < 1)  // no room to copy ahead: rows go by elements
+      launch_norm_grad_block<XT, DT, Any, false, 1024>(a, parts, block, smem, wide, ahead, s);
     else if (threads * groups <= 512)
       launch_norm_grad_block<XT, DT, PT, VEC, 512>(a, parts, block, smem, wide, ahead, s);
     else
@@ -430,10 +430,16 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
   }
 }
 
-template <typename XT, typename DT, typename PT>
+// The weight is read by vectors if its type is f32 or XT, else by elements.
+template <typename XT, typename DT>
 void launch_norm_grad_typed(const NormGradArgs& a, int parts, int vec, cudaStream_t s) {
-  if (vec == VEC_NONE) launch_norm_grad_vec<XT, DT, PT, false>(a, parts, false, s);
-  else launch_norm_grad_vec<XT, DT, PT, true>(a, parts, vec == VEC_32, s);
+  const int type = a.weight ? a.param_type : DMX_TYPE_F32;
+  if (vec != VEC_NONE && type == DMX_TYPE_F32)
+    launch_norm_grad_vec<XT, DT, float, true>(a, parts, vec == VEC_32, s);
+  else if (vec != VEC_NONE && type == type_code(XT()))
+    launch_norm_grad_vec<XT, DT, XT, true>(a, parts, vec == VEC_32, s);
+  else
+    launch_norm_grad_vec<XT, DT, Any, false>(a, parts, false, s);
 }
 
 }  // namespace dmx

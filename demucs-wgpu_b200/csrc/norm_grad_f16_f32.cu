@@ -3,12 +3,8 @@
 
 namespace dmx {
 
-void launch_norm_grad_f16_f32(const NormGradArgs& a, int parts, int vec,
-                             cudaStream_t s) {
-  const int type = a.weight ? a.param_type : DMX_TYPE_F32;
-  if (type == DMX_TYPE_F32) launch_norm_grad_typed<__half, float, float>(a, parts, vec, s);
-  else if (type == DMX_TYPE_F16) launch_norm_grad_typed<__half, float, __half>(a, parts, vec, s);
-  else launch_norm_grad_typed<__half, float, __nv_bfloat16>(a, parts, vec, s);
+void launch_norm_grad_f16_f32(const NormGradArgs& a, int parts, int vec, cudaStream_t s) {
+  launch_norm_grad_typed<__half, float>(a, parts, vec, s);
 }
 
 }  // namespace dmx

@@ -210,6 +210,28 @@ DMX_DEVICE void centre8(float* v, float mean) {
 // How the rows and vectors of a launch may be accessed.
 enum { VEC_NONE = 0, VEC_16 = 1, VEC_32 = 2 };  // by elements; from 16-byte, from 32-byte boundaries
 
+// An array whose type is known only at run time (uniform over the launch), and
+// the tag that stands for its type in templates. Kernels without vector
+// accesses take parameters this way: a third of the instantiations.
+struct Any {};
+struct AnyArray {
+  const void* p;
+  int type;
+  DMX_DEVICE explicit operator bool() const { return p != nullptr; }
+};
+template <typename T>
+DMX_DEVICE const T* array_of(const void* p, int, T) { return static_cast<const T*>(p); }
+DMX_DEVICE AnyArray array_of(const void* p, int type, Any) { return {p, type}; }
+
+// f(T()) for the element type that `type` names (uniform over the launch)
+template <typename F>
+DMX_DEVICE void with_type(int type, F&& f) {
+  if (type == DMX_TYPE_F32) f(float());
+  else if (type == DMX_TYPE_F16) f(__half());
+  else f(__nv_bfloat16());
+}
+DMX_DEVICE float from_bits(uint32_t w, Any) { return __uint_as_float(w); }
+
 // A row is held by `threads` threads in pieces of eight values. Piece j of
 // thread t is, if every row and vector starts on 16 bytes (VEC), the eight
 // neighbours from column (j threads + t) 8 on; else the eight columns
@@ -248,9 +270,17 @@ struct Pieces {
         if (has(j, e)) w[e / kPer] |= ld_bits(p + col(j, e)) << (e % kPer * 16);
     }
   }
+  DMX_DEVICE void fetch(AnyArray p, int j, uint32_t* w) const {  // without VEC
+    with_type(p.type, [&](auto type) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        w[e] = has(j, e) ? __float_as_uint(to_f32(static_cast<const decltype(type)*>(p.p)[col(j, e)]))
+                         : 0;
+    });
+  }
   template <typename T>
   DMX_DEVICE static void unpack(const uint32_t* w, float* v) {
-    if (VEC) {
+    if constexpr (VEC) {
       unpack8(w, v, T());
     } else {
 #pragma unroll
@@ -275,20 +305,15 @@ struct Pieces {
   }
 };
 
-// f(T()) for the element type that `type` names (uniform over the launch)
-template <typename F>
-DMX_DEVICE void with_type(int type, F&& f) {
-  if (type == DMX_TYPE_F32) f(float());
-  else if (type == DMX_TYPE_F16) f(__half());
-  else f(__nv_bfloat16());
-}
-
 // The widest access that suits rows of `ld` elements of `bytes` bytes from p
 // on (ld 0: a vector): 16-bit elements need 16 bytes for eight, f32 ones 32.
 inline int vec_of(const void* p, int64_t ld, int bytes) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * bytes);
   return at % 16 ? VEC_NONE : at % 32 && bytes == 4 ? VEC_16 : VEC_32;
 }
+constexpr int type_code(float) { return DMX_TYPE_F32; }
+constexpr int type_code(__half) { return DMX_TYPE_F16; }
+constexpr int type_code(__nv_bfloat16) { return DMX_TYPE_BF16; }
 inline int type_size(int type) { return type == DMX_TYPE_F32 ? 4 : 2; }
 
 }  // namespace dmx

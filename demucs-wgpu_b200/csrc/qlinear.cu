@@ -313,7 +313,7 @@ DMX_DEVICE void mma_stage(uint32_t d, uint32_t a_addr, uint32_t b_addr, int left
 // up to 128 rows: out^T tile of 128 channels x BT rows per cluster
 // ---------------------------------------------------------------------------
 
-constexpr int kFewThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 read the accumulator
+constexpr int kFewThreads = 512;  // warp 0 TMA, warp 1 MMA, warps 2-5 read the accumulator; all finish
 
 template <int BT, int STAGES>
 struct FewSmem {
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kFewThreads)
   }
   __syncwarp();
   int* part = reinterpret_cast<int*>(smem);  // [BT][128]
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     // lane = channel, column = row of x: [row][channel] is written without bank conflicts
     const int q = warp % 4;
     const bool ok = warp_wait(done, 0, a.err, 13);
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kFewThreads)
     }
     for (int m = split + warp * splits; m < rows; m += kFewThreads / 32 * splits) {
       const int4* at = reinterpret_cast<const int4*>(part + m * 128) + lane;
-      int4 acc = make_int4(0, 0, 0, 0);
+      int4 acc = splits > 1 ? make_int4(0, 0, 0, 0) : *at;
       if (splits > 1) {
         int4 v[8];
 #pragma unroll
@@ -437,8 +437,6 @@ __global__ void __launch_bounds__(kFewThreads)
         for (int p = 0; p < 8; ++p)
           if (p < splits)
             acc = make_int4(acc.x + v[p].x, acc.y + v[p].y, acc.z + v[p].z, acc.w + v[p].w);
-      } else {
-        acc = *at;
       }
       const int64_t row = m0 + m;
       const float xs = a.x_scale ? a.x_scale[row] : 1.f;
@@ -819,7 +817,7 @@ bool launch_few(const LinearArgs& a, cudaStream_t s) {
   const int mtiles = (int)((a.rows + BT - 1) / BT);
   const int blocks = (a.k + kBlockK - 1) / kBlockK;
   int splits = 1;
-  while (splits < 8 && blocks >= splits * 4 && tiles * mtiles * splits * 2 <= 2 * sm_count()) splits *= 2;
+  while (splits < 8 && blocks >= splits * 8 && tiles * mtiles * splits * 2 <= 2 * sm_count()) splits *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * splits), (unsigned)mtiles);
   cfg.blockDim = dim3(kFewThreads);

@@ -147,8 +147,8 @@ template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
 DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const Pieces<VEC>& p,
                                  bool q_vec, float (*sh)[32]) {
   const RowSum<LANES> over;
-  const PT* weight = static_cast<const PT*>(a.weight);
-  const PT* bias = static_cast<const PT*>(a.bias);
+  const auto weight = array_of(a.weight, a.param_type, PT());
+  const auto bias = array_of(a.bias, a.param_type, PT());
   uint32_t raw[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) p.fetch(static_cast<const XT*>(a.x) + row * a.x_ld, j, raw[j]);
@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(1024)
   const int pieces = (a.cols - 1) / ((int)blockDim.x * 8) + 1;
   const int64_t row = blockIdx.x;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
-  const PT* weight = static_cast<const PT*>(a.weight);
-  const PT* bias = static_cast<const PT*>(a.bias);
+  const auto weight = array_of(a.weight, a.param_type, PT());
+  const auto bias = array_of(a.bias, a.param_type, PT());
   float v[8], w[8], mean = 0.f, rstd = 1.f;
   if (MODE != ROWS_QUANTIZE) {
     float s = 0.f;
@@ -322,12 +322,15 @@ __global__ void __launch_bounds__(1024)
     if (MODE != ROWS_QUANTIZE) {
       centre8(v, mean);
       scale8(v, rstd);
+      uint32_t raw[8];
       if (weight) {
-        p.load(weight, j, w);
+        p.fetch(weight, j, raw);
+        Pieces<VEC>::template unpack<PT>(raw, w);
         times8(v, w);
       }
       if (bias) {
-        p.load(bias, j, w);
+        p.fetch(bias, j, raw);
+        Pieces<VEC>::template unpack<PT>(raw, w);
         plus8(v, w);
       }
     } else if (a.col_scale) {
@@ -390,21 +393,28 @@ void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   rows_long_kernel<XT, PT, MODE, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a, wide, q_vec);
 }
 
-template <typename XT, typename PT, int MODE>
-void launch_rows_vec(const RowArgs& a, int vec, bool q_vec, cudaStream_t s) {
-  if (vec == VEC_NONE) launch_rows_mode<XT, PT, MODE, false>(a, false, q_vec, s);
-  else launch_rows_mode<XT, PT, MODE, true>(a, vec == VEC_32, q_vec, s);
-}
-
-template <typename XT, typename PT>
-void launch_rows_norm(const RowArgs& a, cudaStream_t s) {
-  int vec = std::min(vec_of(a.x, a.x_ld, sizeof(XT)),
-                     std::min(vec_of(a.weight, 0, sizeof(PT)), vec_of(a.bias, 0, sizeof(PT))));
-  if (a.y) {
-    vec = std::min(vec, vec_of(a.y, a.y_ld, type_size(a.y_type)));
-    return launch_rows_vec<XT, PT, ROWS_NORM>(a, vec, false, s);
+// MODE on rows of XT; parameters of type f32 or XT are read by vectors, others by elements.
+template <typename XT, int MODE>
+void launch_rows_typed(const RowArgs& a, cudaStream_t s) {
+  int vec = vec_of(a.x, a.x_ld, sizeof(XT));
+  auto narrow = [&vec](const void* p, int64_t ld, int bytes) {
+    vec = std::min(vec, vec_of(p, ld, bytes));
+  };
+  if (MODE == ROWS_NORM) narrow(a.y, a.y_ld, type_size(a.y_type));
+  if (MODE == ROWS_QUANTIZE) {
+    narrow(a.col_scale, 0, 4);
+  } else {
+    narrow(a.weight, 0, type_size(a.param_type));
+    narrow(a.bias, 0, type_size(a.param_type));
   }
-  launch_rows_vec<XT, PT, ROWS_NORM_QUANTIZE>(a, vec, vec_of(a.q, a.q_ld, 1) != VEC_NONE, s);
+  const bool wide = vec == VEC_32, q_vec = vec_of(a.q, a.q_ld, 1) != VEC_NONE;
+  const bool own = a.param_type == type_code(XT()), params = a.weight || a.bias;
+  if (vec != VEC_NONE && MODE != ROWS_QUANTIZE && params && own)
+    launch_rows_mode<XT, XT, MODE, true>(a, wide, q_vec, s);
+  else if (vec != VEC_NONE && (MODE == ROWS_QUANTIZE || !params || a.param_type == DMX_TYPE_F32))
+    launch_rows_mode<XT, float, MODE, true>(a, wide, q_vec, s);
+  else
+    launch_rows_mode<XT, Any, MODE, false>(a, false, q_vec, s);
 }
 
 }  // namespace dmx

@@ -1,11 +1,8 @@
-// The quantiser's row kernels (rows.cuh) on bf16 rows.
+// The row kernels (rows.cuh) of the quantiser on bf16 rows.
 #include "rows.cuh"
 
 namespace dmx {
 
-void launch_rows_quantize_bf16(const RowArgs& a, cudaStream_t s) {
-  const int vec = std::min(vec_of(a.x, a.x_ld, sizeof(__nv_bfloat16)), vec_of(a.col_scale, 0, 4));
-  launch_rows_vec<__nv_bfloat16, float, ROWS_QUANTIZE>(a, vec, vec_of(a.q, a.q_ld, 1) != VEC_NONE, s);
-}
+void launch_rows_quantize_bf16(const RowArgs& a, cudaStream_t s) { launch_rows_typed<__nv_bfloat16, ROWS_QUANTIZE>(a, s); }
 
 }  // namespace dmx

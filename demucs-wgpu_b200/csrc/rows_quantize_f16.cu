@@ -1,11 +1,8 @@
-// The quantiser's row kernels (rows.cuh) on f16 rows.
+// The row kernels (rows.cuh) of the quantiser on f16 rows.
 #include "rows.cuh"
 
 namespace dmx {
 
-void launch_rows_quantize_f16(const RowArgs& a, cudaStream_t s) {
-  const int vec = std::min(vec_of(a.x, a.x_ld, sizeof(__half)), vec_of(a.col_scale, 0, 4));
-  launch_rows_vec<__half, float, ROWS_QUANTIZE>(a, vec, vec_of(a.q, a.q_ld, 1) != VEC_NONE, s);
-}
+void launch_rows_quantize_f16(const RowArgs& a, cudaStream_t s) { launch_rows_typed<__half, ROWS_QUANTIZE>(a, s); }
 
 }  // namespace dmx
