@@ -44,6 +44,8 @@ int parts_of(int64_t rows, int64_t cols, bool vec) {
 __global__ void __launch_bounds__(1024)
     norm_grad_join_kernel(const float* __restrict__ partials, int parts, int cols,
                           float* __restrict__ dweight, float* __restrict__ dbias) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   __shared__ float sh[2][32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float w = 0.f, b = 0.f;
@@ -91,8 +93,8 @@ void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
     launch[a.x_type][a.dy_type](a, parts, vec, s);
   }
   if (sums)
-    norm_grad_join_kernel<<<(a.cols + 31) / 32, 1024, 0, s>>>(a.partials, parts, a.cols, a.dweight,
-                                                             a.dbias);
+    launch_chained(norm_grad_join_kernel, (a.cols + 31) / 32, 1024, 0, s, 1, a.partials, parts, a.cols,
+                   a.dweight, a.dbias);
 }
 
 }  // namespace dmx

@@ -96,6 +96,8 @@ constexpr int kGradThreads = 256;
 template <typename XT, typename DT, typename PT, int LANES, int NV, bool VEC>
 __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
     norm_grad_warp_kernel(const __grid_constant__ NormGradArgs a, bool wide) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   constexpr int per = kGradThreads / LANES, kCols = LANES * NV * 8;
   __shared__ float sums[per][kCols];
   const Pieces<VEC> p = {(int)(threadIdx.x % LANES), LANES, a.cols, wide};
@@ -184,6 +186,8 @@ DMX_DEVICE void copy16(uint32_t dst, const void* src, int bytes) {
 template <typename XT, typename DT, typename PT, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS)
     norm_grad_block_kernel(const __grid_constant__ NormGradArgs a, bool wide, int ahead) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   constexpr int NV = 2, kXUnits = sizeof(XT) / 2, kDUnits = sizeof(DT) / 2;  // of 16 bytes per piece
   constexpr int kStage = NV * (kXUnits + kDUnits);
   extern __shared__ float4 own[];
@@ -324,6 +328,8 @@ __global__ void __launch_bounds__(THREADS)
 template <typename XT, typename DT, typename PT, bool VEC>
 __global__ void __launch_bounds__(1024)
     norm_grad_long_kernel(const __grid_constant__ NormGradArgs a, bool wide) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   __shared__ float2 sh[2][32];
   const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
@@ -365,6 +371,8 @@ __global__ void __launch_bounds__(1024)
 template <typename XT, typename DT, bool VEC>
 __global__ void __launch_bounds__(kGradThreads)
     norm_grad_columns_kernel(const __grid_constant__ NormGradArgs a, bool wide) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   const int pieces = (a.cols - 1) / (kGradThreads * 8) + 1, j = blockIdx.x;
   const Pieces<VEC> p = {(int)threadIdx.x, kGradThreads, a.cols, wide};
   if (j >= pieces || !p.has(j, 0)) return;
@@ -389,22 +397,22 @@ void launch_norm_grad_block(const NormGradArgs& a, int parts, dim3 block, size_t
   static PerDevice once;
   if (once.first())
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-  kernel<<<parts, block, smem, s>>>(a, wide, ahead);
+  launch_chained(kernel, parts, block, smem, s, 1, a, wide, ahead);
 }
 
 // What norm_grad.cu decides: parts (blocks whose partial sums are joined).
 template <typename XT, typename DT, typename PT, bool VEC>
 void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStream_t s) {
   if (a.cols <= 64)
-    norm_grad_warp_kernel<XT, DT, PT, 8, 1, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 8, 1, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
   else if (a.cols <= 128)
-    norm_grad_warp_kernel<XT, DT, PT, 8, 2, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 8, 2, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
   else if (a.cols <= 256)
-    norm_grad_warp_kernel<XT, DT, PT, 16, 2, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 16, 2, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
   else if (a.cols <= 512)
-    norm_grad_warp_kernel<XT, DT, PT, 32, 2, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 32, 2, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
   else if (a.cols <= 1024)
-    norm_grad_warp_kernel<XT, DT, PT, 32, 4, VEC><<<parts, kGradThreads, 0, s>>>(a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 32, 4, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
   else if (a.cols <= kGradBlockCols) {
     const int threads = grad_group_threads(a.cols), groups = grad_groups(a.cols);
     // shared memory per thread: its sums, and the rows to come
@@ -423,10 +431,11 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const unsigned strips = (unsigned)((a.cols - 1) / (kGradThreads * 8) + 1);
     // first: dx may be written over x or dy
     if (a.partials)
-      norm_grad_columns_kernel<XT, DT, VEC><<<dim3(strips, parts), kGradThreads, 0, s>>>(a, wide);
+      launch_chained(norm_grad_columns_kernel<XT, DT, VEC>, dim3(strips, parts), kGradThreads, 0, s, 1, a,
+                     wide);
     if (a.dx)
-      norm_grad_long_kernel<XT, DT, PT, VEC>
-          <<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a, wide);
+      launch_chained(norm_grad_long_kernel<XT, DT, PT, VEC>,
+                     dim3((unsigned)std::min<int64_t>(a.rows, 1 << 20)), 1024, 0, s, 1, a, wide);
   }
 }
 

@@ -305,6 +305,32 @@ struct Pieces {
   }
 };
 
+// The operators' kernels are launched so that one may begin while the kernel
+// before it in the stream still runs (programmatic dependent launch): its
+// blocks set themselves up, then wait here for that kernel's end. Nothing that
+// a kernel before could have written, and nothing at all is written, before
+// after_earlier_kernels() (prefetches into L2 excepted, which fetch no value).
+DMX_DEVICE void let_next_kernel_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
+DMX_DEVICE void after_earlier_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+void launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                    unsigned cluster, A&&... args) {
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim = {cluster, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // The widest access that suits rows of `ld` elements of `bytes` bytes from p
 // on (ld 0: a vector): 16-bit elements need 16 bytes for eight, f32 ones 32.
 inline int vec_of(const void* p, int64_t ld, int bytes) {

@@ -6,9 +6,9 @@
 // Three kernels, all on the same operands (rows on 16-byte boundaries, the
 // bytes past column k of a row never used):
 //  * linear_gemv_kernel: up to 8 rows, dp4a on weights streamed once;
-//  * linear_few_kernel: up to 128 rows, tcgen05 with the weights as the
-//    128-row operand, k split over a thread-block cluster;
-//  * linear_tile_kernel: more rows, persistent tcgen05 tiles of 128 x BN.
+//  * linear_few_kernel: up to 128 rows and long k, tcgen05 with the weights as
+//    the 128-row operand, k split over a thread-block cluster;
+//  * linear_tile_kernel: the rest, persistent tcgen05 tiles.
 #include <algorithm>
 
 #include "ops.h"
@@ -138,17 +138,27 @@ DMX_DEVICE int dot16(int4 x, int4 w, int acc) {
   return __dp4a(x.w, w.w, acc);
 }
 
+DMX_DEVICE void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 constexpr int kGemvThreads = 256;
 
 // A warp takes C channels and every `kw`-th 512-byte piece of k; the `kw`
 // warps of one channel group (8 / kw groups per block) are summed through
 // shared memory. x (at most 8 rows) stays in L1.
 template <int M, int C, typename OT, bool GELU>
-__global__ void __launch_bounds__(kGemvThreads) linear_gemv_kernel(const LinearArgs a, int kw) {
+__global__ void __launch_bounds__(kGemvThreads)
+    linear_gemv_kernel(const __grid_constant__ LinearArgs a, int kw) {
   __shared__ int part[kGemvThreads / 32][M * C];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int groups = (kGemvThreads / 32) / kw, group = warp / kw, kpart = warp % kw;
   const int n0 = (blockIdx.x * groups + group) * C;
+  let_next_kernel_begin();
+  // the weights start towards L2 while the tokens are still being made
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    for (int k0 = (kpart * 32 + lane) * 128; k0 < a.k; k0 += kw * 4096)
+      if (n0 + c < a.n) prefetch_l2(a.w + (int64_t)(n0 + c) * a.w_ld + k0);
+  after_earlier_kernels();
   int acc[M][C];
 #pragma unroll
   for (int m = 0; m < M; ++m)
@@ -291,6 +301,11 @@ DMX_DEVICE bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
 DMX_DEVICE void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 DMX_DEVICE void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+DMX_DEVICE void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0),
+               "r"(c1)
+               : "memory");
+}
 // Every thread of the cluster: shared-memory writes before it are seen after it.
 DMX_DEVICE void cluster_sync() {
   asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
@@ -363,6 +378,10 @@ __global__ void __launch_bounds__(kFewThreads)
 
   const bool elected = elect_one();
   const uint32_t count = (uint32_t)(hi - lo);
+  let_next_kernel_begin();
+  if (warp == 0 && elected)
+    for (int kb = lo; kb < hi; ++kb) tma_prefetch_2d(&tm_w, kb * kBlockK, n0);
+  after_earlier_kernels();
   if (warp == 0) {
     uint32_t it = 0;
     for (int kb = lo; kb < hi; ++kb, ++it) {
@@ -576,6 +595,8 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
   // descriptors then live in uniform registers, which is where the tensor core
   // and the copy engine take them from.
   const bool elected = elect_one();
+  let_next_kernel_begin();
+  after_earlier_kernels();
   if (warp == 0) {
     uint32_t it = 0;
     bool ok = true;
@@ -793,7 +814,7 @@ void launch_gemv(const LinearArgs& a, cudaStream_t s) {
   int kw = 1;
   while (kw < 8 && a.k >= kw * 2048 && (int64_t)a.n * kw < 2ll * 8 * C * sm_count()) kw *= 2;
   const int per = 8 / kw * C;
-  linear_gemv_kernel<M, C, OT, GELU><<<(a.n + per - 1) / per, kGemvThreads, 0, s>>>(a, kw);
+  launch_chained(linear_gemv_kernel<M, C, OT, GELU>, (a.n + per - 1) / per, kGemvThreads, 0, s, 1, a, kw);
 }
 
 // Whether the rows of out and residual start on 16 bytes.
@@ -818,17 +839,8 @@ bool launch_few(const LinearArgs& a, cudaStream_t s) {
   const int blocks = (a.k + kBlockK - 1) / kBlockK;
   int splits = 1;
   while (splits < 8 && blocks >= splits * 8 && tiles * mtiles * splits * 2 <= 2 * sm_count()) splits *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * splits), (unsigned)mtiles);
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = S::TOTAL;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, tw, tx, a, splits, wide_rows<OT>(a));
+  launch_chained(kernel, dim3((unsigned)(tiles * splits), (unsigned)mtiles), kFewThreads, S::TOTAL, s,
+                 (unsigned)splits, tw, tx, a, splits, wide_rows<OT>(a));
   return true;
 }
 
@@ -848,34 +860,29 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
   const TileOrder order = {(uint32_t)mtiles, (uint32_t)ntiles, (uint32_t)(mtiles * ntiles)};
   const int wide = wide_rows<OT>(a);
   const unsigned grid = (unsigned)(kCtas * std::min<int64_t>(mtiles * ntiles, sm_count() / kCtas));
-  if (!S::PAIR) {
-    kernel<<<grid, S::THREADS, S::TOTAL, s>>>(tx, tw, a, order, wide);
-    return true;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(S::THREADS);
-  cfg.dynamicSmemBytes = S::TOTAL;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {kCtas, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, tx, tw, a, order, wide);
+  launch_chained(kernel, grid, S::THREADS, S::TOTAL, s, kCtas, tx, tw, a, order, wide);
   return true;
 }
 
 template <typename OT, bool GELU>
 bool launch_typed(const LinearArgs& a, cudaStream_t s) {
-  if (a.rows <= 8) {
+  // A few rows: dp4a on streamed weights until its multiplications (about a
+  // quarter of what a tensor core's tile start costs per 2^24) outweigh that.
+  // us for 8 rows: 512->512 2.7 against 4.8, 2050->5003 10.1 against 7.2; for 4:
+  // 4096->4096 5.8 against 8.1, 8192->8192 19 against 16.5; one row is always
+  // quicker, 8192->8192 13.6 against 16.3.
+  if (a.rows == 1 || (a.rows <= 8 && a.rows * a.n * a.k <= 1ll << 26)) {
     if (a.rows == 1) launch_gemv<1, 4, OT, GELU>(a, s);
     else if (a.rows == 2) launch_gemv<2, 4, OT, GELU>(a, s);
     else if (a.rows <= 4) launch_gemv<4, 4, OT, GELU>(a, s);
     else launch_gemv<8, 2, OT, GELU>(a, s);
     return true;
   }
-  if (a.rows <= 128) {
+  // k split over a cluster pays where k is long (17 rows, 2048->512: 5.8 us
+  // against 8.0 by tiles; 512->512 5.1 against 4.7) and, past 64 rows, where
+  // tiles would leave most SMs idle (128 rows, 2048->512: 7.6 against 8.2;
+  // 4096->4096 13.5 against 12.6)
+  if (a.k > 1024 && (a.rows <= 64 || (a.rows <= 128 && a.n <= 1024))) {
     if (a.rows <= 16) return launch_few<16, 5, OT, GELU>(a, s);
     if (a.rows <= 32) return launch_few<32, 5, OT, GELU>(a, s);
     if (a.rows <= 64) return launch_few<64, 4, OT, GELU>(a, s);

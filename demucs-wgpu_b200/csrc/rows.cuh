@@ -266,6 +266,8 @@ constexpr int kRowsThreads = 256;
 template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
     rows_warp_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   constexpr int per = kRowsThreads / LANES;
   const int64_t at = (int64_t)blockIdx.x * per + threadIdx.x / LANES;
   const bool live = at < a.rows;
@@ -277,6 +279,8 @@ __global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
 template <typename XT, typename PT, int MODE, int NV, bool VEC>
 __global__ void __launch_bounds__(NV == 4 ? 512 : 1024)
     rows_block_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   __shared__ float sh[3][32];
   const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   row_in_registers<XT, PT, MODE, 0, NV>(a, blockIdx.x, true, p, q_vec, sh);
@@ -286,6 +290,8 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 1024)
 template <typename XT, typename PT, int MODE, bool VEC>
 __global__ void __launch_bounds__(1024)
     rows_long_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
+  let_next_kernel_begin();
+  after_earlier_kernels();
   __shared__ float sh[3][32];
   const RowSum<0> over;
   const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
@@ -366,14 +372,15 @@ __global__ void __launch_bounds__(1024)
 template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
 void launch_rows_warp(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   constexpr int per = kRowsThreads / LANES;
-  rows_warp_kernel<XT, PT, MODE, LANES, NV, VEC>
-      <<<(unsigned)((a.rows + per - 1) / per), kRowsThreads, 0, s>>>(a, wide, q_vec);
+  launch_chained(rows_warp_kernel<XT, PT, MODE, LANES, NV, VEC>,
+                 dim3((unsigned)((a.rows + per - 1) / per)), kRowsThreads, 0, s, 1, a, wide, q_vec);
 }
 
 template <typename XT, typename PT, int MODE, int NV, bool VEC>
 void launch_rows_block(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   const int threads = ((a.cols + NV * 8 - 1) / (NV * 8) + 31) / 32 * 32;
-  rows_block_kernel<XT, PT, MODE, NV, VEC><<<(unsigned)a.rows, threads, 0, s>>>(a, wide, q_vec);
+  launch_chained(rows_block_kernel<XT, PT, MODE, NV, VEC>, dim3((unsigned)a.rows), threads, 0, s, 1, a,
+                 wide, q_vec);
 }
 
 template <typename XT, typename PT, int MODE, bool VEC>
@@ -390,7 +397,8 @@ void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
     if (a.cols <= 2048) return launch_rows_warp<XT, PT, MODE, 32, 8, VEC>(a, wide, q_vec, s);
   constexpr int kBlock = sizeof(XT) == 2 && VEC ? 4 : 2;
   if (a.cols <= 16384) return launch_rows_block<XT, PT, MODE, kBlock, VEC>(a, wide, q_vec, s);
-  rows_long_kernel<XT, PT, MODE, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a, wide, q_vec);
+  launch_chained(rows_long_kernel<XT, PT, MODE, VEC>, dim3((unsigned)a.rows), 1024, 0, s, 1, a, wide,
+                 q_vec);
 }
 
 // MODE on rows of XT; parameters of type f32 or XT are read by vectors, others by elements.
