@@ -93,7 +93,7 @@ void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
     launch[a.x_type][a.dy_type](a, parts, vec, s);
   }
   if (sums)
-    launch_chained(norm_grad_join_kernel, (a.cols + 31) / 32, 1024, 0, s, 1, a.partials, parts, a.cols,
+    launch_chained(norm_grad_join_kernel, (a.cols + 31) / 32, 1024, 0, s, true, 1, a.partials, parts, a.cols,
                    a.dweight, a.dbias);
 }
 

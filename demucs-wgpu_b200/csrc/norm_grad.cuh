@@ -179,11 +179,12 @@ DMX_DEVICE void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
 }
 
-// Rows of up to blockDim.x * 16 columns, a group of blockDim.x threads each;
-// blockDim.y groups to a block. Shared memory, all of it each thread's own and
-// laid out with the thread innermost: the column sums, (dw, db) of two columns
-// to 16 bytes, and with VEC the `ahead` rows to come.
-template <typename XT, typename DT, typename PT, bool VEC, int THREADS>
+// Rows of up to blockDim.x * 16 columns, a group of blockDim.x threads each, R
+// rows at a time (their reductions share their latency); blockDim.y groups to
+// a block. Shared memory, all of it each thread's own and laid out with the
+// thread innermost: the column sums, (dw, db) of two columns to 16 bytes, and
+// with VEC the `ahead` >= R rows to come.
+template <typename XT, typename DT, typename PT, bool VEC, int THREADS, int R>
 __global__ void __launch_bounds__(THREADS)
     norm_grad_block_kernel(const __grid_constant__ NormGradArgs a, bool wide, int ahead) {
   let_next_kernel_begin();
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(THREADS)
   constexpr int NV = 2, kXUnits = sizeof(XT) / 2, kDUnits = sizeof(DT) / 2;  // of 16 bytes per piece
   constexpr int kStage = NV * (kXUnits + kDUnits);
   extern __shared__ float4 own[];
-  __shared__ float2 sh[2][32];
+  __shared__ float2 sh[2][R][32];
   const int n = blockDim.x * blockDim.y, id = threadIdx.y * blockDim.x + threadIdx.x;
   const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   const XT* x = static_cast<const XT*>(a.x);
@@ -237,66 +238,93 @@ __global__ void __launch_bounds__(THREADS)
   for (int j = 0; j < NV; ++j)
     if (weight) p.fetch(weight, j, wraw[j]);
   int turn = 0, stage = 0;
-  for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    uint32_t xraw[NV][8], draw[NV][8];
+  for (int64_t row0 = first; row0 < a.rows; row0 += R * step, turn ^= 1) {
+    uint32_t xraw[R][NV][8], draw[R][NV][8];
+    float mean[R], rstd[R];
+    // every row's copies are a group: the oldest R of `ahead` have landed
     if (VEC) {
-      // every row's copies are a group: the oldest of `ahead` has landed
-      if (ahead == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
-      else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else if (ahead == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      if (ahead == R) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else if (ahead == R + 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else if (ahead == R + 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
       else asm volatile("cp.async.wait_group 3;" ::: "memory");
-      const float4* from = ring + stage * kStage * n;
+    }
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * step;
+      const bool live = R == 1 || row < a.rows;
+      // a row past the last one is zeros and adds nothing
+      mean[r] = live ? a.mean[row] : 0.f;
+      rstd[r] = live ? a.rstd[row] : 0.f;
+      if (VEC) {
+        const float4* from = ring + stage * kStage * n;
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < kXUnits; ++u)
-          *reinterpret_cast<float4*>(&xraw[j][4 * u]) = from[(j * kXUnits + u) * n];
+        for (int j = 0; j < NV; ++j) {
 #pragma unroll
-        for (int u = 0; u < kDUnits; ++u)
-          *reinterpret_cast<float4*>(&draw[j][4 * u]) = from[(NV * kXUnits + j * kDUnits + u) * n];
-      }
-      copy_row(row + ahead * step, stage);
-      stage = stage + 1 == ahead ? 0 : stage + 1;
-    } else {
+          for (int u = 0; u < kXUnits; ++u)
+            *reinterpret_cast<float4*>(&xraw[r][j][4 * u]) = live ? from[(j * kXUnits + u) * n] : none;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        p.fetch(x + row * a.x_ld, j, xraw[j]);
-        p.fetch(dy + row * a.dy_ld, j, draw[j]);
+          for (int u = 0; u < kDUnits; ++u)
+            *reinterpret_cast<float4*>(&draw[r][j][4 * u]) =
+                live ? from[(NV * kXUnits + j * kDUnits + u) * n] : none;
+        }
+        copy_row(row + ahead * step, stage);
+        stage = stage + 1 == ahead ? 0 : stage + 1;
+      } else {
+        const Pieces<VEC> q = {p.t, p.threads, live ? a.cols : 0, wide};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          q.fetch(x + row * a.x_ld, j, xraw[r][j]);
+          q.fetch(dy + row * a.dy_ld, j, draw[r][j]);
+        }
       }
     }
-    float2 s = make_float2(0.f, 0.f);
+    float2 s[R];
     GradPiece<XT, DT, PT, VEC> q;
 #pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = make_float2(0.f, 0.f);
+#pragma unroll
     for (int j = 0; j < NV; ++j) {
-      q.unpack(draw[j], xraw[j], wraw[j], a.weight != nullptr, mean, rstd);
-      s = dot_sums(q.g, q.h, s);
+      float dw[8] = {}, db[8] = {};
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        q.unpack(draw[r][j], xraw[r][j], wraw[j], a.weight != nullptr, mean[r], rstd[r]);
+        s[r] = dot_sums(q.g, q.h, s[r]);
+        gather8(dw, db, q.d, q.h);
+      }
       if (a.partials)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float4* o = &own[(j * 4 + i) * n + id];
-          float4 t = *o;
-          t.x = fmaf(q.d[2 * i], q.h[2 * i], t.x);
-          t.y += q.d[2 * i];
-          t.z = fmaf(q.d[2 * i + 1], q.h[2 * i + 1], t.z);
-          t.w += q.d[2 * i + 1];
-          *o = t;
+          const float4 t = *o;
+          *o = make_float4(t.x + dw[2 * i], t.y + db[2 * i], t.z + dw[2 * i + 1], t.w + db[2 * i + 1]);
         }
     }
     if (!a.dx) continue;
-    s = lanes_sum2<32>(s);
-    // two buffers in turn: the last row's may still be read
-    if (lane == 0) sh[turn][warp] = s;
-    asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
-    s = lanes_sum2<32>(lane < warps ? sh[turn][threadIdx.y * warps + lane] : make_float2(0.f, 0.f));
-    const float m1 = s.x / (float)a.cols, m2 = s.y / (float)a.cols;
-    XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float v[8];
-      q.unpack(draw[j], xraw[j], wraw[j], a.weight != nullptr, mean, rstd);
-      dx8(q.g, q.h, m1, m2, rstd, v);
-      p.store(dx, j, v);
+    for (int r = 0; r < R; ++r) s[r] = lanes_sum2<32>(s[r]);
+    // two buffers in turn: the last rows' may still be read
+    if (lane == 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r) sh[turn][r][warp] = s[r];
+    asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      s[r] = lanes_sum2<32>(lane < warps ? sh[turn][r][threadIdx.y * warps + lane]
+                                         : make_float2(0.f, 0.f));
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * step;
+      if (R > 1 && row >= a.rows) break;
+      const float m1 = s[r].x / (float)a.cols, m2 = s[r].y / (float)a.cols;
+      XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float v[8];
+        q.unpack(draw[r][j], xraw[r][j], wraw[j], a.weight != nullptr, mean[r], rstd[r]);
+        dx8(q.g, q.h, m1, m2, rstd[r], v);
+        p.store(dx, j, v);
+      }
     }
   }
   if (!a.partials) return;
@@ -390,29 +418,29 @@ __global__ void __launch_bounds__(kGradThreads)
   p.store(out + a.cols, j, db);
 }
 
-template <typename XT, typename DT, typename PT, bool VEC, int THREADS>
+template <typename XT, typename DT, typename PT, bool VEC, int THREADS, int R>
 void launch_norm_grad_block(const NormGradArgs& a, int parts, dim3 block, size_t smem, bool wide,
                             int ahead, cudaStream_t s) {
-  auto kernel = norm_grad_block_kernel<XT, DT, PT, VEC, THREADS>;
+  auto kernel = norm_grad_block_kernel<XT, DT, PT, VEC, THREADS, R>;
   static PerDevice once;
   if (once.first())
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-  launch_chained(kernel, parts, block, smem, s, 1, a, wide, ahead);
+  launch_chained(kernel, parts, block, smem, s, true, 1, a, wide, ahead);
 }
 
 // What norm_grad.cu decides: parts (blocks whose partial sums are joined).
 template <typename XT, typename DT, typename PT, bool VEC>
 void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStream_t s) {
   if (a.cols <= 64)
-    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 8, 1, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 8, 1, VEC>, parts, kGradThreads, 0, s, true, 1, a, wide);
   else if (a.cols <= 128)
-    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 8, 2, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 8, 2, VEC>, parts, kGradThreads, 0, s, true, 1, a, wide);
   else if (a.cols <= 256)
-    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 16, 2, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 16, 2, VEC>, parts, kGradThreads, 0, s, true, 1, a, wide);
   else if (a.cols <= 512)
-    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 32, 2, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 32, 2, VEC>, parts, kGradThreads, 0, s, true, 1, a, wide);
   else if (a.cols <= 1024)
-    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 32, 4, VEC>, parts, kGradThreads, 0, s, 1, a, wide);
+    launch_chained(norm_grad_warp_kernel<XT, DT, PT, 32, 4, VEC>, parts, kGradThreads, 0, s, true, 1, a, wide);
   else if (a.cols <= kGradBlockCols) {
     const int threads = grad_group_threads(a.cols), groups = grad_groups(a.cols);
     // shared memory per thread: its sums, and the rows to come
@@ -421,21 +449,24 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const int ahead = VEC ? std::min(4, (most - own) / stage) : 0;
     const dim3 block(threads, groups);
     const size_t smem = (size_t)threads * groups * (own + ahead * stage);
+    // two rows at a time where registers and copies allow it
     if (VEC && ahead < 1)  // no room to copy ahead: rows go by elements
-      launch_norm_grad_block<XT, DT, Any, false, 1024>(a, parts, block, smem, wide, ahead, s);
-    else if (threads * groups <= 512)
-      launch_norm_grad_block<XT, DT, PT, VEC, 512>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, Any, false, 1024, 1>(a, parts, block, smem, wide, ahead, s);
+    else if (threads * groups <= 512 && (!VEC || ahead >= 2))
+      launch_norm_grad_block<XT, DT, PT, VEC, 512, 2>(a, parts, block, smem, wide, ahead, s);
+    else if (threads * groups <= 640 && (!VEC || ahead >= 2))
+      launch_norm_grad_block<XT, DT, PT, VEC, 640, 2>(a, parts, block, smem, wide, ahead, s);
     else
-      launch_norm_grad_block<XT, DT, PT, VEC, 1024>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, VEC, 1024, 1>(a, parts, block, smem, wide, ahead, s);
   } else {
     const unsigned strips = (unsigned)((a.cols - 1) / (kGradThreads * 8) + 1);
     // first: dx may be written over x or dy
     if (a.partials)
-      launch_chained(norm_grad_columns_kernel<XT, DT, VEC>, dim3(strips, parts), kGradThreads, 0, s, 1, a,
+      launch_chained(norm_grad_columns_kernel<XT, DT, VEC>, dim3(strips, parts), kGradThreads, 0, s, true, 1, a,
                      wide);
     if (a.dx)
       launch_chained(norm_grad_long_kernel<XT, DT, PT, VEC>,
-                     dim3((unsigned)std::min<int64_t>(a.rows, 1 << 20)), 1024, 0, s, 1, a, wide);
+                     dim3((unsigned)std::min<int64_t>(a.rows, 1 << 20)), 1024, 0, s, true, 1, a, wide);
   }
 }
 

@@ -814,7 +814,7 @@ void launch_gemv(const LinearArgs& a, cudaStream_t s) {
   int kw = 1;
   while (kw < 8 && a.k >= kw * 2048 && (int64_t)a.n * kw < 2ll * 8 * C * sm_count()) kw *= 2;
   const int per = 8 / kw * C;
-  launch_chained(linear_gemv_kernel<M, C, OT, GELU>, (a.n + per - 1) / per, kGemvThreads, 0, s, 1, a, kw);
+  launch_chained(linear_gemv_kernel<M, C, OT, GELU>, (a.n + per - 1) / per, kGemvThreads, 0, s, true, 1, a, kw);
 }
 
 // Whether the rows of out and residual start on 16 bytes.
@@ -840,7 +840,7 @@ bool launch_few(const LinearArgs& a, cudaStream_t s) {
   int splits = 1;
   while (splits < 8 && blocks >= splits * 8 && tiles * mtiles * splits * 2 <= 2 * sm_count()) splits *= 2;
   launch_chained(kernel, dim3((unsigned)(tiles * splits), (unsigned)mtiles), kFewThreads, S::TOTAL, s,
-                 (unsigned)splits, tw, tx, a, splits, wide_rows<OT>(a));
+                 true, (unsigned)splits, tw, tx, a, splits, wide_rows<OT>(a));
   return true;
 }
 
@@ -860,7 +860,7 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
   const TileOrder order = {(uint32_t)mtiles, (uint32_t)ntiles, (uint32_t)(mtiles * ntiles)};
   const int wide = wide_rows<OT>(a);
   const unsigned grid = (unsigned)(kCtas * std::min<int64_t>(mtiles * ntiles, sm_count() / kCtas));
-  launch_chained(kernel, grid, S::THREADS, S::TOTAL, s, kCtas, tx, tw, a, order, wide);
+  launch_chained(kernel, grid, S::THREADS, S::TOTAL, s, true, kCtas, tx, tw, a, order, wide);
   return true;
 }
 

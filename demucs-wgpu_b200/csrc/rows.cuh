@@ -262,6 +262,7 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
 }
 
 constexpr int kRowsThreads = 256;
+constexpr unsigned kOneRound = 2 * 148;  // blocks that surely run at once
 
 template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
@@ -372,15 +373,16 @@ __global__ void __launch_bounds__(1024)
 template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
 void launch_rows_warp(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   constexpr int per = kRowsThreads / LANES;
-  launch_chained(rows_warp_kernel<XT, PT, MODE, LANES, NV, VEC>,
-                 dim3((unsigned)((a.rows + per - 1) / per)), kRowsThreads, 0, s, 1, a, wide, q_vec);
+  const unsigned grid = (unsigned)((a.rows + per - 1) / per);
+  launch_chained(rows_warp_kernel<XT, PT, MODE, LANES, NV, VEC>, grid, kRowsThreads, 0, s,
+                 grid <= kOneRound, 1, a, wide, q_vec);
 }
 
 template <typename XT, typename PT, int MODE, int NV, bool VEC>
 void launch_rows_block(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   const int threads = ((a.cols + NV * 8 - 1) / (NV * 8) + 31) / 32 * 32;
-  launch_chained(rows_block_kernel<XT, PT, MODE, NV, VEC>, dim3((unsigned)a.rows), threads, 0, s, 1, a,
-                 wide, q_vec);
+  launch_chained(rows_block_kernel<XT, PT, MODE, NV, VEC>, dim3((unsigned)a.rows), threads, 0, s,
+                 a.rows <= kOneRound, 1, a, wide, q_vec);
 }
 
 template <typename XT, typename PT, int MODE, bool VEC>
@@ -397,8 +399,8 @@ void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
     if (a.cols <= 2048) return launch_rows_warp<XT, PT, MODE, 32, 8, VEC>(a, wide, q_vec, s);
   constexpr int kBlock = sizeof(XT) == 2 && VEC ? 4 : 2;
   if (a.cols <= 16384) return launch_rows_block<XT, PT, MODE, kBlock, VEC>(a, wide, q_vec, s);
-  launch_chained(rows_long_kernel<XT, PT, MODE, VEC>, dim3((unsigned)a.rows), 1024, 0, s, 1, a, wide,
-                 q_vec);
+  launch_chained(rows_long_kernel<XT, PT, MODE, VEC>, dim3((unsigned)a.rows), 1024, 0, s,
+                 a.rows <= kOneRound, 1, a, wide, q_vec);
 }
 
 // MODE on rows of XT; parameters of type f32 or XT are read by vectors, others by elements.
