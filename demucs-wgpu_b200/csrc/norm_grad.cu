@@ -48,12 +48,13 @@ __global__ void __launch_bounds__(1024)
   after_earlier_kernels();
   __shared__ float sh[2][32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int64_t pitch = grad_pitch(cols);
   float w = 0.f, b = 0.f;
   if (c < cols)
 #pragma unroll 5
     for (int p = warp; p < parts; p += 32) {
-      w += partials[(int64_t)(2 * p) * cols + c];
-      b += partials[(int64_t)(2 * p + 1) * cols + c];
+      w += partials[2 * p * pitch + c];
+      b += partials[(2 * p + 1) * pitch + c];
     }
   sh[0][warp][lane] = w;
   sh[1][warp][lane] = b;
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(1024)
 
 size_t norm_grad_workspace(int64_t rows, int64_t cols) {
   const int parts = std::max(parts_of(rows, cols, true), parts_of(rows, cols, false));
-  return (size_t)parts * 2 * (size_t)cols * sizeof(float);
+  return (size_t)parts * 2 * (size_t)grad_pitch((int)cols) * sizeof(float);
 }
 
 void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
@@ -80,8 +81,8 @@ void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
   int vec = std::min(vec_of(a.x, a.x_ld, type_size(a.x_type)), vec_of(a.dy, a.dy_ld, type_size(a.dy_type)));
   vec = std::min(vec, vec_of(a.weight, 0, type_size(a.param_type)));
   if (a.dx) vec = std::min(vec, vec_of(a.dx, a.dx_ld, type_size(a.x_type)));
-  // the long rows' partial sums are stored by pieces too
-  if (a.partials && a.cols > kGradBlockCols) vec = std::min(vec, vec_of(a.partials, a.cols, 4));
+  // partial sums of longer rows are stored by pieces too
+  if (a.partials && a.cols > 1024) vec = std::min(vec, vec_of(a.partials, grad_pitch(a.cols), 4));
   const int parts = parts_of(a.rows, a.cols, vec != VEC_NONE);
   if (parts > 0 && (sums || a.dx)) {
     using Launch = void (*)(const NormGradArgs&, int, int, cudaStream_t);

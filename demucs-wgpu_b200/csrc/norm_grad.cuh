@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
   }
   if (!a.partials) return;
   // the block's row groups added in their order
-  float* out = a.partials + (int64_t)blockIdx.x * 2 * a.cols;
+  const int pitch = grad_pitch(a.cols);
+  float* out = a.partials + (int64_t)blockIdx.x * 2 * pitch;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     __syncthreads();
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
       float t = 0.f;
 #pragma unroll
       for (int g = 0; g < per; ++g) t += sums[g][c];
-      out[half * a.cols + c] = t;
+      out[half * pitch + c] = t;
     }
   }
 }
@@ -331,9 +332,11 @@ __global__ void __launch_bounds__(THREADS)
   __syncthreads();
   if (threadIdx.y != 0) return;
   // the block's groups added in their order
-  float* out = a.partials + (int64_t)blockIdx.x * 2 * a.cols;
+  const int pitch = grad_pitch(a.cols);
+  float* out = a.partials + (int64_t)blockIdx.x * 2 * pitch;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    float dw[8], db[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float4 t = own[(j * 4 + i) * n + id];
@@ -341,15 +344,14 @@ __global__ void __launch_bounds__(THREADS)
         const float4 u = own[(j * 4 + i) * n + g * blockDim.x + threadIdx.x];
         t = make_float4(t.x + u.x, t.y + u.y, t.z + u.z, t.w + u.w);
       }
-      if (p.has(j, 2 * i)) {
-        out[p.col(j, 2 * i)] = t.x;
-        out[a.cols + p.col(j, 2 * i)] = t.y;
-      }
-      if (p.has(j, 2 * i + 1)) {
-        out[p.col(j, 2 * i + 1)] = t.z;
-        out[a.cols + p.col(j, 2 * i + 1)] = t.w;
-      }
+      dw[2 * i] = t.x;
+      db[2 * i] = t.y;
+      dw[2 * i + 1] = t.z;
+      db[2 * i + 1] = t.w;
     }
+    p.store(out, j, dw);
+    p.store(out + pitch, j, db);
+  }
 }
 
 // Rows too long for a block's registers: dx, re-reading the row.
@@ -413,9 +415,10 @@ __global__ void __launch_bounds__(kGradThreads)
     scale8(h, a.rstd[row]);
     gather8(dw, db, d, h);
   }
-  float* out = a.partials + (int64_t)blockIdx.y * 2 * a.cols;
+  const int pitch = grad_pitch(a.cols);
+  float* out = a.partials + (int64_t)blockIdx.y * 2 * pitch;
   p.store(out, j, dw);
-  p.store(out + a.cols, j, db);
+  p.store(out + pitch, j, db);
 }
 
 template <typename XT, typename DT, typename PT, bool VEC, int THREADS, int R>

@@ -62,6 +62,8 @@ inline int grad_groups(int cols) {
   const int threads = grad_group_threads(cols);
   return threads >= 512 ? 1 : 512 / threads;
 }
+// Pitch of the partial column sums: whole 32-byte pieces.
+__host__ __device__ inline int grad_pitch(int cols) { return (cols + 7) / 8 * 8; }
 size_t norm_grad_workspace(int64_t rows, int64_t cols);
 void launch_norm_grad(const NormGradArgs& a, cudaStream_t s);
 
