@@ -453,11 +453,11 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const dim3 block(threads, groups);
     const size_t smem = (size_t)threads * groups * (own + ahead * stage);
     // two rows at a time where registers and copies allow it
-    if (VEC && ahead < 1)  // no room to copy ahead: rows go by elements
+    if (!VEC || ahead < 1)  // or no room to copy ahead: rows go by elements
       launch_norm_grad_block<XT, DT, Any, false, 1024, 1>(a, parts, block, smem, wide, ahead, s);
-    else if (threads * groups <= 512 && (!VEC || ahead >= 2))
+    else if (threads * groups <= 512 && ahead >= 2)
       launch_norm_grad_block<XT, DT, PT, VEC, 512, 2>(a, parts, block, smem, wide, ahead, s);
-    else if (threads * groups <= 640 && (!VEC || ahead >= 2))
+    else if (threads * groups <= 640 && ahead >= 2)
       launch_norm_grad_block<XT, DT, PT, VEC, 640, 2>(a, parts, block, smem, wide, ahead, s);
     else
       launch_norm_grad_block<XT, DT, PT, VEC, 1024, 1>(a, parts, block, smem, wide, ahead, s);

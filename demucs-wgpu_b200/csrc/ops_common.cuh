@@ -270,6 +270,41 @@ struct Pieces {
         if (has(j, e)) w[e / kPer] |= ld_bits(p + col(j, e)) << (e % kPer * 16);
     }
   }
+  // The same (VEC) of a row that starts anywhere: the 16-byte units around the
+  // piece, shifted by the row's offset in them. A unit that sticks out of the
+  // row is put together from the row's own elements.
+  template <typename T>
+  DMX_DEVICE void fetch_shifted(const T* p, int j, uint32_t* w) const {
+    constexpr int kSize = sizeof(T), kUnit = 16 / kSize, kUnits = 8 / kUnit + 1, kWords = 4 * kUnits;
+    uint32_t u[kWords + 1];
+    const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);  // uniform over the row
+    const int from = col(j, 0) - off / kSize;                    // first element of the first unit
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int c = from + k * kUnit;
+      if (c >= 0 && c + kUnit <= cols) {
+        ld_words4(p + c, u + 4 * k);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[4 * k + i] = 0;
+        if (c + kUnit > 0 && c < cols) {
+#pragma unroll
+          for (int i = 0; i < kUnit; ++i)
+            if (c + i >= 0 && c + i < cols)
+              u[4 * k + i * kSize / 4] |= ld_bits(p + c + i) << (i * kSize % 4 * 8);
+        }
+      }
+    }
+    u[kWords] = 0;
+    const bool two = off & 8, one = off & 4;
+#pragma unroll
+    for (int i = 0; i + 2 <= kWords; ++i) u[i] = two ? u[i + 2] : u[i];
+#pragma unroll
+    for (int i = 0; i + 1 <= kWords - 2; ++i) u[i] = one ? u[i + 1] : u[i];
+    const int bits = (off & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 2 * kSize; ++i) w[i] = kSize == 4 ? u[i] : __funnelshift_r(u[i], u[i + 1], bits);
+  }
   DMX_DEVICE void fetch(AnyArray p, int j, uint32_t* w) const {  // without VEC
     with_type(p.type, [&](auto type) {
 #pragma unroll

@@ -27,6 +27,9 @@
 namespace dmx {
 
 enum { ROWS_NORM = 0, ROWS_NORM_QUANTIZE = 1, ROWS_QUANTIZE = 2 };
+// How a kernel reads its rows: element by element, by vectors, or (x) by
+// vectors shifted into place.
+enum { BY_ELEMENT = 0, BY_VECTOR = 1, BY_SHIFT = 2 };
 
 // max(|a|, |b|, |c|); a NaN among them comes out as a NaN
 DMX_DEVICE float max3_abs(float a, float b, float c) {
@@ -143,7 +146,7 @@ DMX_DEVICE void mask8(const Pieces<VEC>& p, int j, float* v) {
 
 // One row held in NV pieces per thread; PT is the parameters' type. Without
 // `live` the lanes only take part in the shuffles.
-template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
+template <typename XT, typename PT, int MODE, int LANES, int NV, bool SHIFT, bool VEC>
 DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const Pieces<VEC>& p,
                                  bool q_vec, float (*sh)[32]) {
   const RowSum<LANES> over;
@@ -151,7 +154,11 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
   const auto bias = array_of(a.bias, a.param_type, PT());
   uint32_t raw[NV][8];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) p.fetch(static_cast<const XT*>(a.x) + row * a.x_ld, j, raw[j]);
+  for (int j = 0; j < NV; ++j) {
+    const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
+    if constexpr (SHIFT) p.fetch_shifted(x, j, raw[j]);
+    else p.fetch(x, j, raw[j]);
+  }
   auto get = [&](int j, float* v) { Pieces<VEC>::template unpack<XT>(raw[j], v); };
   float v[8];
   if (MODE == ROWS_QUANTIZE) {
@@ -264,7 +271,7 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
 constexpr int kRowsThreads = 256;
 constexpr unsigned kOneRound = 2 * 148;  // blocks that surely run at once
 
-template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
+template <typename XT, typename PT, int MODE, int LANES, int NV, int VEC>
 __global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
     rows_warp_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
   let_next_kernel_begin();
@@ -273,46 +280,52 @@ __global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
   const int64_t at = (int64_t)blockIdx.x * per + threadIdx.x / LANES;
   const bool live = at < a.rows;
   // lanes without a row hold nothing
-  const Pieces<VEC> p = {(int)(threadIdx.x % LANES), LANES, live ? a.cols : 0, wide};
-  row_in_registers<XT, PT, MODE, LANES, NV>(a, live ? at : 0, live, p, q_vec, nullptr);
+  const Pieces<VEC != BY_ELEMENT> p = {(int)(threadIdx.x % LANES), LANES, live ? a.cols : 0, wide};
+  row_in_registers<XT, PT, MODE, LANES, NV, VEC == BY_SHIFT>(a, live ? at : 0, live, p, q_vec, nullptr);
 }
 
-template <typename XT, typename PT, int MODE, int NV, bool VEC>
+template <typename XT, typename PT, int MODE, int NV, int VEC>
 __global__ void __launch_bounds__(NV == 4 ? 512 : 1024)
     rows_block_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
   let_next_kernel_begin();
   after_earlier_kernels();
   __shared__ float sh[3][32];
-  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
-  row_in_registers<XT, PT, MODE, 0, NV>(a, blockIdx.x, true, p, q_vec, sh);
+  const Pieces<VEC != BY_ELEMENT> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
+  row_in_registers<XT, PT, MODE, 0, NV, VEC == BY_SHIFT>(a, blockIdx.x, true, p, q_vec, sh);
 }
 
 // Rows too long for registers: one block re-reads its row for each reduction.
-template <typename XT, typename PT, int MODE, bool VEC>
+template <typename XT, typename PT, int MODE, int VEC>
 __global__ void __launch_bounds__(1024)
     rows_long_kernel(const __grid_constant__ RowArgs a, bool wide, bool q_vec) {
   let_next_kernel_begin();
   after_earlier_kernels();
   __shared__ float sh[3][32];
   const RowSum<0> over;
-  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
+  const Pieces<VEC != BY_ELEMENT> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   const int pieces = (a.cols - 1) / ((int)blockDim.x * 8) + 1;
   const int64_t row = blockIdx.x;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
   const auto weight = array_of(a.weight, a.param_type, PT());
   const auto bias = array_of(a.bias, a.param_type, PT());
   float v[8], w[8], mean = 0.f, rstd = 1.f;
+  auto load = [&](int j) {
+    uint32_t raw[8];
+    if constexpr (VEC == BY_SHIFT) p.fetch_shifted(x, j, raw);
+    else p.fetch(x, j, raw);
+    p.template unpack<XT>(raw, v);
+  };
   if (MODE != ROWS_QUANTIZE) {
     float s = 0.f;
     for (int j = 0; j < pieces; ++j) {
-      p.load(x, j, v);
+      load(j);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += v[e];
     }
     mean = over.sum(s, sh[0]) / (float)a.cols;
     s = 0.f;
     for (int j = 0; j < pieces; ++j) {
-      p.load(x, j, v);
+      load(j);
       centre8(v, mean);
       mask8(p, j, v);
 #pragma unroll
@@ -325,19 +338,19 @@ __global__ void __launch_bounds__(1024)
     }
   }
   auto value = [&](int j) {
-    p.load(x, j, v);
+    load(j);
     if (MODE != ROWS_QUANTIZE) {
       centre8(v, mean);
       scale8(v, rstd);
       uint32_t raw[8];
       if (weight) {
         p.fetch(weight, j, raw);
-        Pieces<VEC>::template unpack<PT>(raw, w);
+        Pieces<VEC != BY_ELEMENT>::template unpack<PT>(raw, w);
         times8(v, w);
       }
       if (bias) {
         p.fetch(bias, j, raw);
-        Pieces<VEC>::template unpack<PT>(raw, w);
+        Pieces<VEC != BY_ELEMENT>::template unpack<PT>(raw, w);
         plus8(v, w);
       }
     } else if (a.col_scale) {
@@ -370,7 +383,7 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-template <typename XT, typename PT, int MODE, int LANES, int NV, bool VEC>
+template <typename XT, typename PT, int MODE, int LANES, int NV, int VEC>
 void launch_rows_warp(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   constexpr int per = kRowsThreads / LANES;
   const unsigned grid = (unsigned)((a.rows + per - 1) / per);
@@ -378,14 +391,14 @@ void launch_rows_warp(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
                  grid <= kOneRound, 1, a, wide, q_vec);
 }
 
-template <typename XT, typename PT, int MODE, int NV, bool VEC>
+template <typename XT, typename PT, int MODE, int NV, int VEC>
 void launch_rows_block(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   const int threads = ((a.cols + NV * 8 - 1) / (NV * 8) + 31) / 32 * 32;
   launch_chained(rows_block_kernel<XT, PT, MODE, NV, VEC>, dim3((unsigned)a.rows), threads, 0, s,
                  a.rows <= kOneRound, 1, a, wide, q_vec);
 }
 
-template <typename XT, typename PT, int MODE, bool VEC>
+template <typename XT, typename PT, int MODE, int VEC>
 void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   // a few rows: as many threads as there are pieces, for the shortest chain
   if (a.cols > 256 && a.cols <= 8192 && a.rows <= 2 * sm_count())
@@ -395,9 +408,9 @@ void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
   if (a.cols <= 256) return launch_rows_warp<XT, PT, MODE, 8, 4, VEC>(a, wide, q_vec, s);
   if (a.cols <= 512) return launch_rows_warp<XT, PT, MODE, 16, 4, VEC>(a, wide, q_vec, s);
   if (a.cols <= 1024) return launch_rows_warp<XT, PT, MODE, 32, 4, VEC>(a, wide, q_vec, s);
-  if constexpr (sizeof(XT) == 2 && MODE != ROWS_NORM_QUANTIZE && VEC)
+  if constexpr (sizeof(XT) == 2 && MODE != ROWS_NORM_QUANTIZE && VEC != BY_ELEMENT)
     if (a.cols <= 2048) return launch_rows_warp<XT, PT, MODE, 32, 8, VEC>(a, wide, q_vec, s);
-  constexpr int kBlock = sizeof(XT) == 2 && VEC ? 4 : 2;
+  constexpr int kBlock = sizeof(XT) == 2 && VEC != BY_ELEMENT ? 4 : 2;
   if (a.cols <= 16384) return launch_rows_block<XT, PT, MODE, kBlock, VEC>(a, wide, q_vec, s);
   launch_chained(rows_long_kernel<XT, PT, MODE, VEC>, dim3((unsigned)a.rows), 1024, 0, s,
                  a.rows <= kOneRound, 1, a, wide, q_vec);
@@ -406,7 +419,7 @@ void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
 // MODE on rows of XT; parameters of type f32 or XT are read by vectors, others by elements.
 template <typename XT, int MODE>
 void launch_rows_typed(const RowArgs& a, cudaStream_t s) {
-  int vec = vec_of(a.x, a.x_ld, sizeof(XT));
+  int vec = VEC_32;  // of all operands but x
   auto narrow = [&vec](const void* p, int64_t ld, int bytes) {
     vec = std::min(vec, vec_of(p, ld, bytes));
   };
@@ -417,14 +430,26 @@ void launch_rows_typed(const RowArgs& a, cudaStream_t s) {
     narrow(a.weight, 0, type_size(a.param_type));
     narrow(a.bias, 0, type_size(a.param_type));
   }
-  const bool wide = vec == VEC_32, q_vec = vec_of(a.q, a.q_ld, 1) != VEC_NONE;
-  const bool own = a.param_type == type_code(XT()), params = a.weight || a.bias;
-  if (vec != VEC_NONE && MODE != ROWS_QUANTIZE && params && own)
-    launch_rows_mode<XT, XT, MODE, true>(a, wide, q_vec, s);
-  else if (vec != VEC_NONE && (MODE == ROWS_QUANTIZE || !params || a.param_type == DMX_TYPE_F32))
-    launch_rows_mode<XT, float, MODE, true>(a, wide, q_vec, s);
-  else
-    launch_rows_mode<XT, Any, MODE, false>(a, false, q_vec, s);
+  const int x_vec = vec_of(a.x, a.x_ld, sizeof(XT));
+  const bool wide = std::min(vec, x_vec) == VEC_32, q_vec = vec_of(a.q, a.q_ld, 1) != VEC_NONE;
+  const bool params = a.weight || a.bias;
+  const bool as_f32 = MODE == ROWS_QUANTIZE || !params || a.param_type == DMX_TYPE_F32;
+  const bool as_xt = params && a.param_type == type_code(XT());
+  if (vec == VEC_NONE || !(as_f32 || as_xt))
+    return launch_rows_mode<XT, Any, MODE, BY_ELEMENT>(a, false, q_vec, s);
+  if (x_vec == VEC_NONE) {
+    // x alone starts off 16 bytes, as rows of an odd length do before they are
+    // quantised: its units are shifted into place
+    if constexpr (MODE != ROWS_NORM) {
+      if (as_f32) launch_rows_mode<XT, float, MODE, BY_SHIFT>(a, vec == VEC_32, q_vec, s);
+      else launch_rows_mode<XT, XT, MODE, BY_SHIFT>(a, vec == VEC_32, q_vec, s);
+    } else {
+      launch_rows_mode<XT, Any, MODE, BY_ELEMENT>(a, false, q_vec, s);
+    }
+    return;
+  }
+  if (as_f32) launch_rows_mode<XT, float, MODE, BY_VECTOR>(a, wide, q_vec, s);
+  else launch_rows_mode<XT, XT, MODE, BY_VECTOR>(a, wide, q_vec, s);
 }
 
 }  // namespace dmx
