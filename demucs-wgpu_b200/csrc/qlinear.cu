@@ -493,8 +493,8 @@ __global__ void __launch_bounds__(kFewThreads)
 
 constexpr int kGroupRows = 8;  // row tiles per group of the tile order
 
-// Warp 0 issues TMA, warp 1 the MMAs, the others are the epilogue: four, one
-// per quarter of the accumulator's lanes, for every 64 columns. Tiles of 256
+// Warp 0 issues TMA, warp 1 the MMAs, the other 16 are the epilogue: four, one
+// per quarter of the accumulator's lanes, for each quarter of the columns. Tiles of 256
 // columns are worked on by a pair of CTAs, 128 rows each, which halves what
 // each of them loads of w: with a CTA alone, its shared memory took in 48 KB
 // and gave out as much for every 512 cycles of the tensor core, more than L2
@@ -503,10 +503,11 @@ template <int BN>
 struct Tile {
   static constexpr bool PAIR = BN == 256;
   static constexpr int ROWS = PAIR ? 256 : 128;
-  static constexpr int EPI_WARPS = BN / 16, THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int EPI_WARPS = 16, THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int WIDTH = BN / 4;  // an epilogue warp's columns
   static constexpr int A = 128 * kBlockK, B = BN * kBlockK / (PAIR ? 2 : 1), STAGE = A + B;
   static constexpr int TURN = EPI_WARPS * 4096;       // epilogue warps' outputs on their way
-  static constexpr int COLUMN = EPI_WARPS * 64 * 8;   // their channel scales and biases
+  static constexpr int COLUMN = EPI_WARPS * WIDTH * 8;  // their channel scales and biases
   static constexpr int STAGES = (227 * 1024 - TURN - COLUMN - 1024 - 256) / STAGE;
   static constexpr int TOTAL = STAGES * STAGE + TURN + COLUMN + 1024 + 256;
   static constexpr uint32_t COLS = 2 * BN;
@@ -524,26 +525,130 @@ struct TileOrder {
   }
 };
 
-// One epilogue warp's 32 rows x 64 columns of a tile, a lane holding a row,
-// to memory by whole 128-byte lines: through 4 KB of shared memory in which the
-// 16-byte units of row r are permuted by r % 8, so that neither the rows'
-// writes nor the lines' reads meet in a bank. (Stores of 32 bytes to each of 32
-// rows ran at 2.1 TB/s for 16-bit outputs, 2.9 for f32 ones.)
+// One epilogue warp's 32 rows of a tile, a lane holding a row, to memory by
+// whole lines: through 4 KB of shared memory in which the 16-byte units of row
+// r are permuted by r % 8, so that neither the rows' writes nor the lines'
+// reads meet in a bank. (Stores of 32 bytes to each of 32 rows ran at 2.1 TB/s
+// for 16-bit outputs, 2.9 for f32 ones.)
 template <typename OT>
 struct Lines {
   unsigned char* buf;  // 32 rows of 128 bytes
   int lane;
   DMX_DEVICE void* unit(int row, int u) const { return buf + row * 128 + ((u ^ (row & 7)) << 4); }
   // 8 / 4 values of this lane's row as unit u
-  DMX_DEVICE void put_packed(int u, const float* v) const {
+  DMX_DEVICE void put_packed(int u, const float2* v) const {
     *reinterpret_cast<uint4*>(unit(lane, u)) =
-        make_uint4(pack2(v[0], v[1], OT()), pack2(v[2], v[3], OT()), pack2(v[4], v[5], OT()),
-                   pack2(v[6], v[7], OT()));
+        make_uint4(pack2(v[0].x, v[0].y, OT()), pack2(v[1].x, v[1].y, OT()),
+                   pack2(v[2].x, v[2].y, OT()), pack2(v[3].x, v[3].y, OT()));
   }
-  DMX_DEVICE void put_f32(int u, const float* v) const {
-    *reinterpret_cast<float4*>(unit(lane, u)) = make_float4(v[0], v[1], v[2], v[3]);
+  DMX_DEVICE void put_f32(int u, const float2* v) const {
+    *reinterpret_cast<float4*>(unit(lane, u)) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
   }
 };
+
+// 16 columns of a row of the accumulator, scaled (col: two columns' scales and
+// biases to 16 bytes) and activated.
+template <bool GELU>
+DMX_DEVICE void tile_values(uint32_t tmem_at, const float4* col, float row_scale, float2* v) {
+  uint32_t r[16];
+  tmem_ld16_nw(tmem_at, r);
+  tmem_ld_wait<16>(r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 q = col[i];
+    v[i] = scaled2((int)r[2 * i], (int)r[2 * i + 1], row_scale, make_float2(q.x, q.y),
+                   make_float2(q.z, q.w));
+  }
+  if (GELU) gelu_pairs<8>(v);
+}
+
+// An epilogue warp's share of a tile: `rows` of its 32 rows exist, from row m0
+// and column n0 of the output on.
+template <int WIDTH, typename OT, bool GELU>
+DMX_DEVICE void tile_share(const LinearArgs& a, const Lines<OT>& lines, uint32_t tmem_at, const float4* col,
+                           float row_scale, int64_t m0, int n0, int rows, bool wide) {
+  const int lane = lines.lane;
+  OT* out = static_cast<OT*>(a.out) + m0 * a.out_ld + n0;
+  // unrolled, the GELU's coefficients are set up once; without a GELU the loads of
+  // several turns at once only spilled registers (112896x128->2048: 200 us against 131)
+  constexpr int kUnroll = GELU ? 4 : 1;
+  if constexpr (sizeof(OT) == 2) {
+    if (!a.residual) {  // rounded before they cross: all columns in one pass
+#pragma unroll kUnroll
+      for (int c = 0; c < WIDTH; c += 16) {
+        float2 v[8];
+        tile_values<GELU>(tmem_at + c, col + c / 2, row_scale, v);
+        lines.put_packed(c / 8, v);
+        lines.put_packed(c / 8 + 1, v + 4);
+      }
+      __syncwarp();
+      if (wide && n0 + WIDTH <= a.n) {
+        constexpr int kUnits = WIDTH / 8;
+        OT* at = out + (lane / kUnits) * a.out_ld + (lane % kUnits) * 8;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int row = 32 / kUnits * i + lane / kUnits;
+          const uint4 w = *reinterpret_cast<const uint4*>(lines.unit(row, lane % kUnits));
+          if (row < rows) st_words4(at, reinterpret_cast<const uint32_t*>(&w));
+          at += 32 / kUnits * a.out_ld;
+        }
+      } else {  // rows that do not start on 16 bytes, or end here: by elements
+        const int cols = min(WIDTH, a.n - n0);
+        for (int row = 0; row < rows; ++row)
+          for (int c = lane; c < cols; c += 32)
+            out[row * a.out_ld + c] = static_cast<const OT*>(lines.unit(row, c / 8))[c % 8];
+      }
+      __syncwarp();
+      return;
+    }
+  }
+  // as f32, 32 columns to a pass; a residual is added after the crossing
+  constexpr int kPass = WIDTH < 32 ? WIDTH : 32, kUnits = kPass / 4;
+#pragma unroll 1
+  for (int p = 0; p < WIDTH && n0 + p < a.n; p += kPass) {
+    const bool whole = wide && n0 + p + kPass <= a.n;
+    const OT* residual = static_cast<const OT*>(a.residual) + m0 * a.residual_ld + n0 + p;
+    float4 q[kUnits];
+    if (whole && a.residual) {  // on its way while the accumulator is read
+      const OT* at = residual + (lane / kUnits) * a.residual_ld + (lane % kUnits) * 4;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        if (32 / kUnits * i + lane / kUnits < rows) q[i] = load4(at);
+        at += 32 / kUnits * a.residual_ld;
+      }
+    }
+#pragma unroll kUnroll
+    for (int c = 0; c < kPass; c += 16) {
+      float2 v[8];
+      tile_values<GELU>(tmem_at + p + c, col + (p + c) / 2, row_scale, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lines.put_f32(c / 4 + i, v + 2 * i);
+    }
+    __syncwarp();
+    if (whole) {
+      OT* at = out + p + (lane / kUnits) * a.out_ld + (lane % kUnits) * 4;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int row = 32 / kUnits * i + lane / kUnits;
+        float4 f = *reinterpret_cast<const float4*>(lines.unit(row, lane % kUnits));
+        if (row < rows) {
+          if (a.residual) f = make_float4(f.x + q[i].x, f.y + q[i].y, f.z + q[i].z, f.w + q[i].w);
+          store4(at, f);
+        }
+        at += 32 / kUnits * a.out_ld;
+      }
+    } else {
+      const int cols = min(kPass, a.n - n0 - p);
+      for (int row = 0; row < rows; ++row)
+        for (int c = lane; c < cols; c += 32) {
+          float f = static_cast<const float*>(lines.unit(row, c / 4))[c % 4];
+          if (a.residual) f += to_f32(residual[row * a.residual_ld + c]);
+          out[row * a.out_ld + p + c] = from_f32<OT>(f);
+        }
+    }
+    __syncwarp();
+  }
+}
 
 template <int BN, typename OT, bool GELU>
 __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
@@ -649,15 +754,16 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
     }
     if (!ok && elected) drain_mmas<PAIR>(drain, a.err);
   } else {
-    // this warp: rows 32 quarter + lane, columns c_lo .. c_lo + 63 of each tile
-    const int quarter = warp % 4, c_lo = (warp - 2) / 4 * 64;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    // this warp: rows 32 quarter + lane, columns c_lo .. c_lo + WIDTH - 1 of each tile
+    constexpr int WIDTH = S::WIDTH;
+    const int quarter = warp % 4, c_lo = (warp - 2) / 4 * WIDTH;
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + c_lo;
     const Lines<OT> lines = {turn + (warp - 2) * 4096, lane};
     // its channel scales and biases, two columns to 16 bytes. A tile's are
     // fetched while the tile before it is worked on, each warp its own: no
     // barrier among the epilogue's warps, which so drift apart and share the
     // issue slots with one another's waits.
-    float4* col = column + (warp - 2) * 32;
+    float4* col = column + (warp - 2) * (WIDTH / 2);
     float4 sb;
     float xs;
     int64_t m0_next;
@@ -665,20 +771,26 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
     auto fetch = [&](uint32_t t) {
       uint32_t mt, nt;
       order.at(t, mt, nt);
-      m0_next = (int64_t)mt * S::ROWS + rank * 128;
-      n0_next = (int)(nt * BN);
-      const int n = n0_next + c_lo + 2 * lane;
+      m0_next = (int64_t)mt * S::ROWS + rank * 128 + quarter * 32;
+      n0_next = (int)(nt * BN) + c_lo;
+      const int n = n0_next + 2 * lane;
       sb = make_float4(1.f, 1.f, 0.f, 0.f);
-      if (a.w_scale) {
-        if (n < a.n) sb.x = a.w_scale[n];
-        if (n + 1 < a.n) sb.y = a.w_scale[n + 1];
+      if (2 * lane < WIDTH) {
+        if (a.w_scale) {
+          if (n < a.n) sb.x = a.w_scale[n];
+          if (n + 1 < a.n) sb.y = a.w_scale[n + 1];
+        }
+        if (a.bias) {
+          if (n < a.n) sb.z = a.bias[n];
+          if (n + 1 < a.n) sb.w = a.bias[n + 1];
+        }
       }
-      if (a.bias) {
-        if (n < a.n) sb.z = a.bias[n];
-        if (n + 1 < a.n) sb.w = a.bias[n + 1];
-      }
-      const int64_t m = m0_next + quarter * 32 + lane;
+      const int64_t m = m0_next + lane;
       xs = m < a.rows && a.x_scale ? a.x_scale[m] : 1.f;
+      if (a.residual && m < a.rows) {  // towards L2: this row's share of the residual
+        const OT* at = static_cast<const OT*>(a.residual) + m * a.residual_ld + n0_next;
+        for (int c = 0; c < WIDTH && n0_next + c < a.n; c += 128 / (int)sizeof(OT)) prefetch_l2(at + c);
+      }
     };
     bool ok = true;
     int tl = 0;
@@ -688,92 +800,14 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
       const int n0 = n0_next, acc = tl & 1;
       const float row_scale = xs;
       __syncwarp();
-      col[lane] = sb;
+      if (2 * lane < WIDTH) col[lane] = sb;
       __syncwarp();
       if (t + step < order.total) fetch(t + step);
       ok = ok && warp_wait(&acc_full[acc], (tl >> 1) & 1, a.err, 24);
       tc_after_sync();
-      if (ok) {
-        const int rows = (int)min((int64_t)32, a.rows - m0 - quarter * 32);
-        // columns of one pass through the lines: 16-bit outputs go rounded, 64 to
-        // a line; where a residual is added first they go as f32, as f32 ones do
-        const bool packed = sizeof(OT) == 2 && !a.residual;
-#pragma unroll 1
-        for (int c0 = c_lo; c0 < c_lo + 64 && n0 + c0 < a.n; c0 += 16) {
-          uint32_t r[16];
-          tmem_ld16_nw(tmem + lanes + (uint32_t)(acc * BN + c0), r);
-          tmem_ld_wait<16>(r);
-          float2 v2[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 q = col[(c0 - c_lo) / 2 + i];
-            v2[i] = scaled2((int)r[2 * i], (int)r[2 * i + 1], row_scale, make_float2(q.x, q.y),
-                            make_float2(q.z, q.w));
-          }
-          if (GELU) gelu_pairs<8>(v2);
-          float v[16];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[2 * i] = v2[i].x;
-            v[2 * i + 1] = v2[i].y;
-          }
-          if constexpr (sizeof(OT) == 2) {
-            if (packed) {
-              lines.put_packed((c0 & 63) / 8, v);
-              lines.put_packed((c0 & 63) / 8 + 1, v + 8);
-            }
-          }
-          if (!packed) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) lines.put_f32((c0 & 31) / 4 + i, v + 4 * i);
-          }
-          // the pass is full, or the matrix ends here
-          const int span = packed ? 64 : 32, first = c0 & ~(span - 1);
-          if ((c0 & (span - 1)) + 16 < span && n0 + c0 + 16 < a.n) continue;
-          __syncwarp();
-          const int n = n0 + first, cols = min(span, a.n - n);
-          OT* out = static_cast<OT*>(a.out) + (m0 + quarter * 32) * a.out_ld + n;
-          const OT* residual = static_cast<const OT*>(a.residual) +
-                               (m0 + quarter * 32) * a.residual_ld + n;
-          if (packed && wide && cols == 64) {
-            if constexpr (sizeof(OT) == 2) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int row = 4 * i + lane / 8;
-                const uint4 w = *reinterpret_cast<const uint4*>(lines.unit(row, lane & 7));
-                if (row < rows)
-                  st_words4(out + row * a.out_ld + (lane & 7) * 8, reinterpret_cast<const uint32_t*>(&w));
-              }
-            }
-          } else if (!packed && wide && cols == 32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = 4 * i + lane / 8;
-              float4 f = *reinterpret_cast<const float4*>(lines.unit(row, lane & 7));
-              if (row < rows) {
-                if (a.residual) {
-                  const float4 q = load4(residual + row * a.residual_ld + (lane & 7) * 4);
-                  f = make_float4(f.x + q.x, f.y + q.y, f.z + q.z, f.w + q.w);
-                }
-                store4(out + row * a.out_ld + (lane & 7) * 4, f);
-              }
-            }
-          } else {
-            // rows that do not start on 16 bytes, or end in this pass: by elements
-            for (int row = 0; row < rows; ++row)
-              for (int c = lane; c < cols; c += 32) {
-                float f;
-                if (packed)
-                  f = to_f32(static_cast<const OT*>(lines.unit(row, c / 8))[c % 8]);
-                else
-                  f = static_cast<const float*>(lines.unit(row, c / 4))[c % 4];
-                if (a.residual) f += to_f32(residual[row * a.residual_ld + c]);
-                out[row * a.out_ld + c] = from_f32<OT>(f);
-              }
-          }
-          __syncwarp();
-        }
-      }
+      if (ok && n0 < a.n)
+        tile_share<WIDTH, OT, GELU>(a, lines, from + (uint32_t)(acc * BN), col, row_scale, m0, n0,
+                                    (int)min((int64_t)32, a.rows - m0), wide);
       tc_before_sync();
       __syncwarp();
       if (lane == 0) {
