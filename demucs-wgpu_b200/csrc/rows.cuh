@@ -187,9 +187,9 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
     }
     return;
   }
-  // one piece per thread is the form for a few rows, where a load's latency
-  // counts: the parameters are fetched with the row
-  constexpr bool kEarly = NV == 1;
+  // the forms for a few rows, where a load's latency counts, fetch the
+  // parameters with the row
+  constexpr bool kEarly = NV == 1 || (LANES == 32 && NV == 2);
   constexpr int kHold = kEarly ? NV : 1;
   uint32_t wr[kHold][8], br[kHold][8];
   if (kEarly) {
@@ -400,8 +400,13 @@ void launch_rows_block(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) 
 
 template <typename XT, typename PT, int MODE, int VEC>
 void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
-  // a few rows: as many threads as there are pieces, for the shortest chain
-  if (a.cols > 256 && a.cols <= 8192 && a.rows <= 2 * sm_count())
+  // few rows: more threads to a row, for the shortest chain (2688x512 f32 normed
+  // and quantised: 5.5 us by 16 lanes with 4 pieces)
+  if (a.rows <= 32 * sm_count()) {
+    if (a.cols > 128 && a.cols <= 256) return launch_rows_warp<XT, PT, MODE, 32, 1, VEC>(a, wide, q_vec, s);
+    if (a.cols > 256 && a.cols <= 512) return launch_rows_warp<XT, PT, MODE, 32, 2, VEC>(a, wide, q_vec, s);
+  }
+  if (a.cols > 512 && a.cols <= 8192 && a.rows <= (VEC == BY_ELEMENT ? 8 : 2) * sm_count())
     return launch_rows_block<XT, PT, MODE, 1, VEC>(a, wide, q_vec, s);
   if (a.cols <= 64) return launch_rows_warp<XT, PT, MODE, 8, 1, VEC>(a, wide, q_vec, s);
   if (a.cols <= 128) return launch_rows_warp<XT, PT, MODE, 8, 2, VEC>(a, wide, q_vec, s);
