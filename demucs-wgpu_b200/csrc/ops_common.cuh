@@ -340,6 +340,26 @@ struct Pieces {
   }
 };
 
+// Eight values of each lane to rows that start anywhere: through `buf` (1 KB, a
+// warp's own), so that a warp's one-element stores are neighbours. LANES lanes
+// share a row, whose columns from `col0` on are the first one's; `row0` is the
+// warp's first row. Every lane takes part.
+template <int LANES, typename T>
+DMX_DEVICE void store_crossed(T* buf, const float* v, T* out, int64_t ld, int64_t row0, int64_t rows,
+                              int col0, int cols) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) buf[lane * 8 + e] = from_f32<T>(v[e]);
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int at = e * 32 + lane, c = col0 + at % (LANES * 8);
+    const int64_t row = row0 + at / (LANES * 8);
+    if (row < rows && c < cols) out[row * ld + c] = buf[at];
+  }
+  __syncwarp();
+}
+
 // The operators' kernels are launched so that one may begin while the kernel
 // before it in the stream still runs (programmatic dependent launch): its
 // blocks set themselves up, then wait here for that kernel's end. Nothing that

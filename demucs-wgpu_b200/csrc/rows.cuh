@@ -27,8 +27,8 @@
 namespace dmx {
 
 enum { ROWS_NORM = 0, ROWS_NORM_QUANTIZE = 1, ROWS_QUANTIZE = 2 };
-// How a kernel reads its rows: element by element, by vectors, or (x) by
-// vectors shifted into place.
+// How a kernel reads its rows: element by element, by vectors, or (rows that
+// start off 16 bytes) by vectors shifted into place.
 enum { BY_ELEMENT = 0, BY_VECTOR = 1, BY_SHIFT = 2 };
 
 // max(|a|, |b|, |c|); a NaN among them comes out as a NaN
@@ -144,11 +144,13 @@ DMX_DEVICE void mask8(const Pieces<VEC>& p, int j, float* v) {
   }
 }
 
+constexpr int kRowsThreads = 256;
+
 // One row held in NV pieces per thread; PT is the parameters' type. Without
 // `live` the lanes only take part in the shuffles.
 template <typename XT, typename PT, int MODE, int LANES, int NV, bool SHIFT, bool VEC>
 DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const Pieces<VEC>& p,
-                                 bool q_vec, float (*sh)[32]) {
+                                 bool q_vec, float (*sh)[32], float* cross) {
   const RowSum<LANES> over;
   const auto weight = array_of(a.weight, a.param_type, PT());
   const auto bias = array_of(a.bias, a.param_type, PT());
@@ -242,6 +244,21 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
     }
   };
   if (MODE == ROWS_NORM) {
+    if constexpr (SHIFT) {
+      constexpr int kLanes = LANES ? LANES : 32;
+      const int64_t row0 = LANES ? (int64_t)blockIdx.x * (kRowsThreads / kLanes) + threadIdx.x / 32 * (32 / kLanes) : row;
+      with_type(a.y_type, [&](auto type) {
+        using T = decltype(type);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          value(j, v);
+          store_crossed<kLanes>(reinterpret_cast<T*>(cross + threadIdx.x / 32 * 256), v,
+                                static_cast<T*>(a.y), a.y_ld, row0, LANES ? a.rows : row + 1,
+                                (j * p.threads + p.t / kLanes * kLanes) * 8, a.cols);
+        }
+      });
+      return;
+    }
     if (!live) return;
     with_type(a.y_type, [&](auto type) {
       auto* y = static_cast<decltype(type)*>(a.y) + row * a.y_ld;
@@ -268,7 +285,6 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
   for (int j = 0; j < NV; ++j) quant.store(a.q + row * a.q_ld, p, q_vec, j, y[j]);
 }
 
-constexpr int kRowsThreads = 256;
 constexpr unsigned kOneRound = 2 * 148;  // blocks that surely run at once
 
 template <typename XT, typename PT, int MODE, int LANES, int NV, int VEC>
@@ -281,7 +297,8 @@ __global__ void __launch_bounds__(kRowsThreads, NV == 8 ? 3 : 1)
   const bool live = at < a.rows;
   // lanes without a row hold nothing
   const Pieces<VEC != BY_ELEMENT> p = {(int)(threadIdx.x % LANES), LANES, live ? a.cols : 0, wide};
-  row_in_registers<XT, PT, MODE, LANES, NV, VEC == BY_SHIFT>(a, live ? at : 0, live, p, q_vec, nullptr);
+  __shared__ float cross[VEC == BY_SHIFT && MODE == ROWS_NORM ? kRowsThreads * 8 : 1];
+  row_in_registers<XT, PT, MODE, LANES, NV, VEC == BY_SHIFT>(a, live ? at : 0, live, p, q_vec, nullptr, cross);
 }
 
 template <typename XT, typename PT, int MODE, int NV, int VEC>
@@ -290,8 +307,10 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 1024)
   let_next_kernel_begin();
   after_earlier_kernels();
   __shared__ float sh[3][32];
+  constexpr int kMost = NV == 4 ? 512 : 1024;
+  __shared__ float cross[VEC == BY_SHIFT && MODE == ROWS_NORM ? kMost * 8 : 1];
   const Pieces<VEC != BY_ELEMENT> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
-  row_in_registers<XT, PT, MODE, 0, NV, VEC == BY_SHIFT>(a, blockIdx.x, true, p, q_vec, sh);
+  row_in_registers<XT, PT, MODE, 0, NV, VEC == BY_SHIFT>(a, blockIdx.x, true, p, q_vec, sh, cross);
 }
 
 // Rows too long for registers: one block re-reads its row for each reduction.
@@ -359,11 +378,17 @@ __global__ void __launch_bounds__(1024)
     }
   };
   if (MODE == ROWS_NORM) {
+    __shared__ float cross[VEC == BY_SHIFT && MODE == ROWS_NORM ? 1024 * 8 : 1];
     with_type(a.y_type, [&](auto type) {
-      auto* y = static_cast<decltype(type)*>(a.y) + row * a.y_ld;
+      using T = decltype(type);
       for (int j = 0; j < pieces; ++j) {
         value(j);
-        p.store(y, j, v);
+        if constexpr (VEC == BY_SHIFT)
+          store_crossed<32>(reinterpret_cast<T*>(cross + threadIdx.x / 32 * 256), v,
+                            static_cast<T*>(a.y), a.y_ld, row, row + 1,
+                            (j * p.threads + p.t / 32 * 32) * 8, a.cols);
+        else
+          p.store(static_cast<T*>(a.y) + row * a.y_ld, j, v);
       }
     });
     return;
@@ -424,33 +449,29 @@ void launch_rows_mode(const RowArgs& a, bool wide, bool q_vec, cudaStream_t s) {
 // MODE on rows of XT; parameters of type f32 or XT are read by vectors, others by elements.
 template <typename XT, int MODE>
 void launch_rows_typed(const RowArgs& a, cudaStream_t s) {
-  int vec = VEC_32;  // of all operands but x
+  int vec = VEC_32;  // of the parameters
   auto narrow = [&vec](const void* p, int64_t ld, int bytes) {
     vec = std::min(vec, vec_of(p, ld, bytes));
   };
-  if (MODE == ROWS_NORM) narrow(a.y, a.y_ld, type_size(a.y_type));
   if (MODE == ROWS_QUANTIZE) {
     narrow(a.col_scale, 0, 4);
   } else {
     narrow(a.weight, 0, type_size(a.param_type));
     narrow(a.bias, 0, type_size(a.param_type));
   }
-  const int x_vec = vec_of(a.x, a.x_ld, sizeof(XT));
-  const bool wide = std::min(vec, x_vec) == VEC_32, q_vec = vec_of(a.q, a.q_ld, 1) != VEC_NONE;
+  int row_vec = vec_of(a.x, a.x_ld, sizeof(XT));
+  if (MODE == ROWS_NORM) row_vec = std::min(row_vec, vec_of(a.y, a.y_ld, type_size(a.y_type)));
+  const bool wide = std::min(vec, row_vec) == VEC_32, q_vec = vec_of(a.q, a.q_ld, 1) != VEC_NONE;
   const bool params = a.weight || a.bias;
   const bool as_f32 = MODE == ROWS_QUANTIZE || !params || a.param_type == DMX_TYPE_F32;
   const bool as_xt = params && a.param_type == type_code(XT());
   if (vec == VEC_NONE || !(as_f32 || as_xt))
     return launch_rows_mode<XT, Any, MODE, BY_ELEMENT>(a, false, q_vec, s);
-  if (x_vec == VEC_NONE) {
-    // x alone starts off 16 bytes, as rows of an odd length do before they are
-    // quantised: its units are shifted into place
-    if constexpr (MODE != ROWS_NORM) {
-      if (as_f32) launch_rows_mode<XT, float, MODE, BY_SHIFT>(a, vec == VEC_32, q_vec, s);
-      else launch_rows_mode<XT, XT, MODE, BY_SHIFT>(a, vec == VEC_32, q_vec, s);
-    } else {
-      launch_rows_mode<XT, Any, MODE, BY_ELEMENT>(a, false, q_vec, s);
-    }
+  if (row_vec == VEC_NONE) {
+    // rows start off 16 bytes, as those of an odd length do: x's units are
+    // shifted into place, a norm's outputs cross between lanes
+    if (as_f32) launch_rows_mode<XT, float, MODE, BY_SHIFT>(a, vec == VEC_32, q_vec, s);
+    else launch_rows_mode<XT, XT, MODE, BY_SHIFT>(a, vec == VEC_32, q_vec, s);
     return;
   }
   if (as_f32) launch_rows_mode<XT, float, MODE, BY_VECTOR>(a, wide, q_vec, s);
