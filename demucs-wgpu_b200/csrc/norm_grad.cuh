@@ -206,29 +206,29 @@ __global__ void __launch_bounds__(THREADS)
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  // this thread's units of a row: where they start (bytes) and how much of them exists
+  int x_from[NV * kXUnits], x_bytes[NV * kXUnits], d_from[NV * kDUnits], d_bytes[NV * kDUnits];
+  auto units = [&](int size, int per, int* from, int* bytes) {
+#pragma unroll
+    for (int i = 0; i < NV * per; ++i) {
+      const int at = p.col(i / per, 0) * size + i % per * 16;
+      bytes[i] = min(max(a.cols * size - at, 0), 16);
+      from[i] = bytes[i] ? at : 0;
+    }
+  };
+  units(sizeof(XT), kXUnits, x_from, x_bytes);
+  units(sizeof(DT), kDUnits, d_from, d_bytes);
   // the copies of one row into stage s of the ring; an empty group past the end
   auto copy_row = [&](int64_t row, int s) {
     if (row < a.rows) {
       const uint32_t at = ring_at + (uint32_t)(s * kStage * n) * 16;
+      const char* xs = reinterpret_cast<const char*>(x + row * a.x_ld);
+      const char* ds = reinterpret_cast<const char*>(dy + row * a.dy_ld);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = p.col(j, 0);
-        const XT* xs = x + row * a.x_ld;
-        const DT* ds = dy + row * a.dy_ld;
+      for (int i = 0; i < NV * kXUnits; ++i) copy16(at + (uint32_t)(i * n) * 16, xs + x_from[i], x_bytes[i]);
 #pragma unroll
-        for (int u = 0; u < kXUnits; ++u) {
-          const int from = c + u * (16 / (int)sizeof(XT));
-          const int bytes = min(max((a.cols - from) * (int)sizeof(XT), 0), 16);
-          copy16(at + (uint32_t)((j * kXUnits + u) * n) * 16, xs + (bytes ? from : 0), bytes);
-        }
-#pragma unroll
-        for (int u = 0; u < kDUnits; ++u) {
-          const int from = c + u * (16 / (int)sizeof(DT));
-          const int bytes = min(max((a.cols - from) * (int)sizeof(DT), 0), 16);
-          copy16(at + (uint32_t)((NV * kXUnits + j * kDUnits + u) * n) * 16, ds + (bytes ? from : 0),
-                 bytes);
-        }
-      }
+      for (int i = 0; i < NV * kDUnits; ++i)
+        copy16(at + (uint32_t)((NV * kXUnits + i) * n) * 16, ds + d_from[i], d_bytes[i]);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -239,9 +239,26 @@ __global__ void __launch_bounds__(THREADS)
   for (int j = 0; j < NV; ++j)
     if (weight) p.fetch(weight, j, wraw[j]);
   int turn = 0, stage = 0;
+  // a row past the last one is zeros and adds nothing
+  float mean_next[R], rstd_next[R];
+  auto fetch_stats = [&](int64_t row0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = row0 + r * step < a.rows;
+      mean_next[r] = live ? a.mean[row0 + r * step] : 0.f;
+      rstd_next[r] = live ? a.rstd[row0 + r * step] : 0.f;
+    }
+  };
+  fetch_stats(first);
   for (int64_t row0 = first; row0 < a.rows; row0 += R * step, turn ^= 1) {
     uint32_t xraw[R][NV][8], draw[R][NV][8];
     float mean[R], rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = mean_next[r];
+      rstd[r] = rstd_next[r];
+    }
+    fetch_stats(row0 + R * step);
     // every row's copies are a group: the oldest R of `ahead` have landed
     if (VEC) {
       if (ahead == R) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -253,9 +270,6 @@ __global__ void __launch_bounds__(THREADS)
     for (int r = 0; r < R; ++r) {
       const int64_t row = row0 + r * step;
       const bool live = R == 1 || row < a.rows;
-      // a row past the last one is zeros and adds nothing
-      mean[r] = live ? a.mean[row] : 0.f;
-      rstd[r] = live ? a.rstd[row] : 0.f;
       if (VEC) {
         const float4* from = ring + stage * kStage * n;
         const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -453,14 +467,16 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const dim3 block(threads, groups);
     const size_t smem = (size_t)threads * groups * (own + ahead * stage);
     // two rows at a time where registers and copies allow it
-    if (!VEC || ahead < 1)  // or no room to copy ahead: rows go by elements
+    if constexpr (!VEC)
+      launch_norm_grad_block<XT, DT, PT, false, 1024, 1>(a, parts, block, smem, wide, ahead, s);
+    else if (ahead < 1)  // no room to copy ahead: rows go by elements
       launch_norm_grad_block<XT, DT, Any, false, 1024, 1>(a, parts, block, smem, wide, ahead, s);
     else if (threads * groups <= 512 && ahead >= 2)
-      launch_norm_grad_block<XT, DT, PT, VEC, 512, 2>(a, parts, block, smem, wide, ahead, s);
-    else if (threads * groups <= 640 && ahead >= 2)
-      launch_norm_grad_block<XT, DT, PT, VEC, 640, 2>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, true, 512, 2>(a, parts, block, smem, wide, ahead, s);
+    else if (threads * groups <= 640)
+      launch_norm_grad_block<XT, DT, PT, true, 640, 1>(a, parts, block, smem, wide, ahead, s);
     else
-      launch_norm_grad_block<XT, DT, PT, VEC, 1024, 1>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, true, 1024, 1>(a, parts, block, smem, wide, ahead, s);
   } else {
     const unsigned strips = (unsigned)((a.cols - 1) / (kGradThreads * 8) + 1);
     // first: dx may be written over x or dy
