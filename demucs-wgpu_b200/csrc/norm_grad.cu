@@ -8,7 +8,7 @@
 
 namespace dmx {
 
-#define DMX_GRAD_UNIT(x) void launch_norm_grad_##x(const NormGradArgs& a, int parts, int vec, cudaStream_t s);
+#define DMX_GRAD_UNIT(x) void launch_norm_grad_##x(const NormGradArgs& a, int parts, int how, bool wide, cudaStream_t s);
 DMX_GRAD_UNIT(f32_f32)
 DMX_GRAD_UNIT(f32_f16)
 DMX_GRAD_UNIT(f32_bf16)
@@ -78,20 +78,23 @@ void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
   NormGradArgs a = args;
   const bool sums = a.dweight || a.dbias;
   if (!sums) a.partials = nullptr;
-  int vec = std::min(vec_of(a.x, a.x_ld, type_size(a.x_type)), vec_of(a.dy, a.dy_ld, type_size(a.dy_type)));
-  vec = std::min(vec, vec_of(a.weight, 0, type_size(a.param_type)));
-  if (a.dx) vec = std::min(vec, vec_of(a.dx, a.dx_ld, type_size(a.x_type)));
+  int row_vec = std::min(vec_of(a.x, a.x_ld, type_size(a.x_type)), vec_of(a.dy, a.dy_ld, type_size(a.dy_type)));
+  if (a.dx) row_vec = std::min(row_vec, vec_of(a.dx, a.dx_ld, type_size(a.x_type)));
+  int vec = vec_of(a.weight, 0, type_size(a.param_type));
   // partial sums of longer rows are stored by pieces too
   if (a.partials && a.cols > 1024) vec = std::min(vec, vec_of(a.partials, grad_pitch(a.cols), 4));
-  const int parts = parts_of(a.rows, a.cols, vec != VEC_NONE);
+  const bool wide = std::min(vec, row_vec) == VEC_32;
+  int how = vec == VEC_NONE || row_vec == VEC_NONE ? BY_ELEMENT : BY_VECTOR;
+  if (vec != VEC_NONE && row_vec == VEC_NONE && a.cols > 1024 && a.cols <= kGradBlockCols) how = BY_SHIFT;
+  const int parts = parts_of(a.rows, a.cols, how == BY_VECTOR);
   if (parts > 0 && (sums || a.dx)) {
-    using Launch = void (*)(const NormGradArgs&, int, int, cudaStream_t);
+    using Launch = void (*)(const NormGradArgs&, int, int, bool, cudaStream_t);
     // by dmx_type of x and of dy: F32, F16, BF16
     static const Launch launch[3][3] = {
         {launch_norm_grad_f32_f32, launch_norm_grad_f32_f16, launch_norm_grad_f32_bf16},
         {launch_norm_grad_f16_f32, launch_norm_grad_f16_f16, launch_norm_grad_f16_bf16},
         {launch_norm_grad_bf16_f32, launch_norm_grad_bf16_f16, launch_norm_grad_bf16_bf16}};
-    launch[a.x_type][a.dy_type](a, parts, vec, s);
+    launch[a.x_type][a.dy_type](a, parts, how, how == BY_SHIFT ? vec == VEC_32 : wide, s);
   }
   if (sums)
     launch_chained(norm_grad_join_kernel, (a.cols + 31) / 32, 1024, 0, s, true, 1, a.partials, parts, a.cols,

@@ -183,9 +183,10 @@ DMX_DEVICE void copy16(uint32_t dst, const void* src, int bytes) {
 // Rows of up to blockDim.x * 16 columns, a group of blockDim.x threads each, R
 // rows at a time (their reductions share their latency); blockDim.y groups to
 // a block. Shared memory, all of it each thread's own and laid out with the
-// thread innermost: the column sums, (dw, db) of two columns to 16 bytes, and
-// with VEC the `ahead` >= R rows to come.
-template <typename XT, typename DT, typename PT, bool VEC, int THREADS, int R>
+// thread innermost: the column sums, (dw, db) of two columns to 16 bytes, and,
+// BY_VECTOR, the `ahead` >= R rows to come. BY_SHIFT, rows that start off 16
+// bytes: read by shifted vectors, dx written across lanes.
+template <typename XT, typename DT, typename PT, int VEC, int THREADS, int R>
 __global__ void __launch_bounds__(THREADS)
     norm_grad_block_kernel(const __grid_constant__ NormGradArgs a, bool wide, int ahead) {
   let_next_kernel_begin();
@@ -194,8 +195,9 @@ __global__ void __launch_bounds__(THREADS)
   constexpr int kStage = NV * (kXUnits + kDUnits);
   extern __shared__ float4 own[];
   __shared__ float2 sh[2][R][32];
+  __shared__ float cross[VEC == BY_SHIFT ? THREADS * 8 : 1];
   const int n = blockDim.x * blockDim.y, id = threadIdx.y * blockDim.x + threadIdx.x;
-  const Pieces<VEC> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
+  const Pieces<VEC != BY_ELEMENT> p = {(int)threadIdx.x, (int)blockDim.x, a.cols, wide};
   const XT* x = static_cast<const XT*>(a.x);
   const DT* dy = static_cast<const DT*>(a.dy);
   const auto weight = array_of(a.weight, a.param_type, PT());
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(THREADS)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (VEC)
+  if (VEC == BY_VECTOR)
     for (int s = 0; s < ahead; ++s) copy_row(first + s * step, s);
   uint32_t wraw[NV][8];
 #pragma unroll
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(THREADS)
     }
     fetch_stats(row0 + R * step);
     // every row's copies are a group: the oldest R of `ahead` have landed
-    if (VEC) {
+    if (VEC == BY_VECTOR) {
       if (ahead == R) asm volatile("cp.async.wait_group 0;" ::: "memory");
       else if (ahead == R + 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
       else if (ahead == R + 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(THREADS)
     for (int r = 0; r < R; ++r) {
       const int64_t row = row0 + r * step;
       const bool live = R == 1 || row < a.rows;
-      if (VEC) {
+      if (VEC == BY_VECTOR) {
         const float4* from = ring + stage * kStage * n;
         const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -286,16 +288,21 @@ __global__ void __launch_bounds__(THREADS)
         copy_row(row + ahead * step, stage);
         stage = stage + 1 == ahead ? 0 : stage + 1;
       } else {
-        const Pieces<VEC> q = {p.t, p.threads, live ? a.cols : 0, wide};
+        const Pieces<VEC != BY_ELEMENT> q = {p.t, p.threads, live ? a.cols : 0, wide};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          q.fetch(x + row * a.x_ld, j, xraw[r][j]);
-          q.fetch(dy + row * a.dy_ld, j, draw[r][j]);
+          if constexpr (VEC == BY_SHIFT) {
+            q.fetch_shifted(x + row * a.x_ld, j, xraw[r][j]);
+            q.fetch_shifted(dy + row * a.dy_ld, j, draw[r][j]);
+          } else {
+            q.fetch(x + row * a.x_ld, j, xraw[r][j]);
+            q.fetch(dy + row * a.dy_ld, j, draw[r][j]);
+          }
         }
       }
     }
     float2 s[R];
-    GradPiece<XT, DT, PT, VEC> q;
+    GradPiece<XT, DT, PT, VEC != BY_ELEMENT> q;
 #pragma unroll
     for (int r = 0; r < R; ++r) s[r] = make_float2(0.f, 0.f);
 #pragma unroll
@@ -338,7 +345,11 @@ __global__ void __launch_bounds__(THREADS)
         float v[8];
         q.unpack(draw[r][j], xraw[r][j], wraw[j], a.weight != nullptr, mean[r], rstd[r]);
         dx8(q.g, q.h, m1, m2, rstd[r], v);
-        p.store(dx, j, v);
+        if constexpr (VEC == BY_SHIFT)
+          store_crossed<32>(reinterpret_cast<XT*>(cross + id / 32 * 256), v, static_cast<XT*>(a.dx),
+                            a.dx_ld, row, row + 1, (j * p.threads + p.t / 32 * 32) * 8, a.cols);
+        else
+          p.store(dx, j, v);
       }
     }
   }
@@ -435,14 +446,23 @@ __global__ void __launch_bounds__(kGradThreads)
   p.store(out + pitch, j, db);
 }
 
-template <typename XT, typename DT, typename PT, bool VEC, int THREADS, int R>
+template <typename XT, typename DT, typename PT, int VEC, int THREADS, int R>
 void launch_norm_grad_block(const NormGradArgs& a, int parts, dim3 block, size_t smem, bool wide,
                             int ahead, cudaStream_t s) {
   auto kernel = norm_grad_block_kernel<XT, DT, PT, VEC, THREADS, R>;
   static PerDevice once;
   if (once.first())
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         (VEC == BY_SHIFT ? 128 : 220) * 1024);
   launch_chained(kernel, parts, block, smem, s, true, 1, a, wide, ahead);
+}
+
+// Long rows that start off 16 bytes, the weight and the partial sums on them.
+template <typename XT, typename DT, typename PT>
+void launch_norm_grad_shift(const NormGradArgs& a, int parts, bool wide, cudaStream_t s) {
+  const int threads = grad_group_threads(a.cols), groups = grad_groups(a.cols);
+  launch_norm_grad_block<XT, DT, PT, BY_SHIFT, 1024, 1>(a, parts, dim3(threads, groups),
+                                                        (size_t)threads * groups * 128, wide, 0, s);
 }
 
 // What norm_grad.cu decides: parts (blocks whose partial sums are joined).
@@ -468,15 +488,15 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const size_t smem = (size_t)threads * groups * (own + ahead * stage);
     // two rows at a time where registers and copies allow it
     if constexpr (!VEC)
-      launch_norm_grad_block<XT, DT, PT, false, 1024, 1>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, BY_ELEMENT, 1024, 1>(a, parts, block, smem, wide, ahead, s);
     else if (ahead < 1)  // no room to copy ahead: rows go by elements
-      launch_norm_grad_block<XT, DT, Any, false, 1024, 1>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, Any, BY_ELEMENT, 1024, 1>(a, parts, block, smem, wide, ahead, s);
     else if (threads * groups <= 512 && ahead >= 2)
-      launch_norm_grad_block<XT, DT, PT, true, 512, 2>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, BY_VECTOR, 512, 2>(a, parts, block, smem, wide, ahead, s);
     else if (threads * groups <= 640)
-      launch_norm_grad_block<XT, DT, PT, true, 640, 1>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, BY_VECTOR, 640, 1>(a, parts, block, smem, wide, ahead, s);
     else
-      launch_norm_grad_block<XT, DT, PT, true, 1024, 1>(a, parts, block, smem, wide, ahead, s);
+      launch_norm_grad_block<XT, DT, PT, BY_VECTOR, 1024, 1>(a, parts, block, smem, wide, ahead, s);
   } else {
     const unsigned strips = (unsigned)((a.cols - 1) / (kGradThreads * 8) + 1);
     // first: dx may be written over x or dy
@@ -491,14 +511,14 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
 
 // The weight is read by vectors if its type is f32 or XT, else by elements.
 template <typename XT, typename DT>
-void launch_norm_grad_typed(const NormGradArgs& a, int parts, int vec, cudaStream_t s) {
+void launch_norm_grad_typed(const NormGradArgs& a, int parts, int how, bool wide, cudaStream_t s) {
   const int type = a.weight ? a.param_type : DMX_TYPE_F32;
-  if (vec != VEC_NONE && type == DMX_TYPE_F32)
-    launch_norm_grad_vec<XT, DT, float, true>(a, parts, vec == VEC_32, s);
-  else if (vec != VEC_NONE && type == type_code(XT()))
-    launch_norm_grad_vec<XT, DT, XT, true>(a, parts, vec == VEC_32, s);
-  else
-    launch_norm_grad_vec<XT, DT, Any, false>(a, parts, false, s);
+  const bool as_f32 = type == DMX_TYPE_F32, as_xt = type == type_code(XT());
+  if (how == BY_VECTOR && as_f32) launch_norm_grad_vec<XT, DT, float, true>(a, parts, wide, s);
+  else if (how == BY_VECTOR && as_xt) launch_norm_grad_vec<XT, DT, XT, true>(a, parts, wide, s);
+  else if (how == BY_SHIFT && as_f32) launch_norm_grad_shift<XT, DT, float>(a, parts, wide, s);
+  else if (how == BY_SHIFT && as_xt) launch_norm_grad_shift<XT, DT, XT>(a, parts, wide, s);
+  else launch_norm_grad_vec<XT, DT, Any, false>(a, parts, false, s);
 }
 
 }  // namespace dmx

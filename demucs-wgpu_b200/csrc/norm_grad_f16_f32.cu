@@ -3,8 +3,8 @@
 
 namespace dmx {
 
-void launch_norm_grad_f16_f32(const NormGradArgs& a, int parts, int vec, cudaStream_t s) {
-  launch_norm_grad_typed<__half, float>(a, parts, vec, s);
+void launch_norm_grad_f16_f32(const NormGradArgs& a, int parts, int how, bool wide, cudaStream_t s) {
+  launch_norm_grad_typed<__half, float>(a, parts, how, wide, s);
 }
 
 }  // namespace dmx

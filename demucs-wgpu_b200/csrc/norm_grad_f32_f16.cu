@@ -3,8 +3,8 @@
 
 namespace dmx {
 
-void launch_norm_grad_f32_f16(const NormGradArgs& a, int parts, int vec, cudaStream_t s) {
-  launch_norm_grad_typed<float, __half>(a, parts, vec, s);
+void launch_norm_grad_f32_f16(const NormGradArgs& a, int parts, int how, bool wide, cudaStream_t s) {
+  launch_norm_grad_typed<float, __half>(a, parts, how, wide, s);
 }
 
 }  // namespace dmx

@@ -207,6 +207,10 @@ DMX_DEVICE void centre8(float* v, float mean) {
   }
 }
 
+// How a kernel reads its rows: element by element, by vectors, or (rows that
+// start off 16 bytes) by vectors shifted into place.
+enum { BY_ELEMENT = 0, BY_VECTOR = 1, BY_SHIFT = 2 };
+
 // How the rows and vectors of a launch may be accessed.
 enum { VEC_NONE = 0, VEC_16 = 1, VEC_32 = 2 };  // by elements; from 16-byte, from 32-byte boundaries
 

@@ -27,9 +27,6 @@
 namespace dmx {
 
 enum { ROWS_NORM = 0, ROWS_NORM_QUANTIZE = 1, ROWS_QUANTIZE = 2 };
-// How a kernel reads its rows: element by element, by vectors, or (rows that
-// start off 16 bytes) by vectors shifted into place.
-enum { BY_ELEMENT = 0, BY_VECTOR = 1, BY_SHIFT = 2 };
 
 // max(|a|, |b|, |c|); a NaN among them comes out as a NaN
 DMX_DEVICE float max3_abs(float a, float b, float c) {

@@ -384,7 +384,7 @@ def test_layer_norm_gradients_match_differences(ops, rows, cols):
 
 
 @pytest.mark.parametrize("which", ["dy", "x"])
-@pytest.mark.parametrize("cols", [500, 2048, 17000])
+@pytest.mark.parametrize("cols", [500, 2048, 3001, 17000])
 def test_layer_norm_backward_in_place(ops, which, cols):
     import torch
 
