@@ -42,8 +42,7 @@ int parts_of(int64_t rows, int64_t cols, bool vec) {
 // 32 columns per block; each of its 32 warps adds a share of the parts, whose
 // sums are joined in order.
 __global__ void __launch_bounds__(1024)
-    norm_grad_join_kernel(const float* __restrict__ partials, int parts, int cols,
-                          float* __restrict__ dweight, float* __restrict__ dbias) {
+    norm_grad_join_kernel(const float* partials, int parts, int cols, float* dweight, float* dbias) {
   let_next_kernel_begin();
   after_earlier_kernels();
   __shared__ float sh[2][32][33];

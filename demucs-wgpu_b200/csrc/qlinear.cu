@@ -9,6 +9,10 @@
 //  * linear_few_kernel: up to 128 rows and long k, tcgen05 with the weights as
 //    the 128-row operand, k split over a thread-block cluster;
 //  * linear_tile_kernel: the rest, persistent tcgen05 tiles.
+// The first two are bound by the weights' bytes (1 x 8192 -> 8192: 13.6 us, 4.9
+// TB/s), the last by the tensor core where k is long (8192^3: 358 us, 3.07
+// POP/s) and by its epilogue or HBM where it is short (112896 x 512 -> 2048 to
+// bf16: 150 us; with GELU 214).
 #include <algorithm>
 
 #include "ops.h"
@@ -119,7 +123,9 @@ DMX_DEVICE void store_out(const LinearArgs& a, int64_t m, int n, float v) {
 DMX_DEVICE int4 row16(const int8_t* row, int k0, int k) {
   int4 v = make_int4(0, 0, 0, 0);
   if (k0 >= k) return v;
-  v = __ldg(reinterpret_cast<const int4*>(row + k0));
+  // not by the read-only path: what a kernel before writes is written while
+  // this one, begun early, already runs
+  v = *reinterpret_cast<const int4*>(row + k0);
   const int left = k - k0;
   if (left < 16) {
     int* w = reinterpret_cast<int*>(&v);
@@ -153,11 +159,12 @@ __global__ void __launch_bounds__(kGemvThreads)
   const int groups = (kGemvThreads / 32) / kw, group = warp / kw, kpart = warp % kw;
   const int n0 = (blockIdx.x * groups + group) * C;
   let_next_kernel_begin();
-  // the weights start towards L2 while the tokens are still being made
+  // the first weights start towards L2 while the tokens are still being made
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    for (int k0 = (kpart * 32 + lane) * 128; k0 < a.k; k0 += kw * 4096)
-      if (n0 + c < a.n) prefetch_l2(a.w + (int64_t)(n0 + c) * a.w_ld + k0);
+  for (int c = 0; c < C; ++c) {
+    const int k0 = (kpart * 32 + lane) * 128;
+    if (n0 + c < a.n && k0 < a.k) prefetch_l2(a.w + (int64_t)(n0 + c) * a.w_ld + k0);
+  }
   after_earlier_kernels();
   int acc[M][C];
 #pragma unroll
@@ -380,7 +387,7 @@ __global__ void __launch_bounds__(kFewThreads)
   const uint32_t count = (uint32_t)(hi - lo);
   let_next_kernel_begin();
   if (warp == 0 && elected)
-    for (int kb = lo; kb < hi; ++kb) tma_prefetch_2d(&tm_w, kb * kBlockK, n0);
+    for (int kb = lo; kb < min(hi, lo + STAGES); ++kb) tma_prefetch_2d(&tm_w, kb * kBlockK, n0);
   after_earlier_kernels();
   if (warp == 0) {
     uint32_t it = 0;
@@ -570,7 +577,7 @@ DMX_DEVICE void tile_share(const LinearArgs& a, const Lines<OT>& lines, uint32_t
   const int lane = lines.lane;
   OT* out = static_cast<OT*>(a.out) + m0 * a.out_ld + n0;
   // unrolled, the GELU's coefficients are set up once; without a GELU the loads of
-  // several turns at once only spilled registers (112896x128->2048: 200 us against 131)
+  // several turns at once only spilled registers (112896x512->2048: 220 us against 150)
   constexpr int kUnroll = GELU ? 4 : 1;
   if constexpr (sizeof(OT) == 2) {
     if (!a.residual) {  // rounded before they cross: all columns in one pass
@@ -900,22 +907,21 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
 
 template <typename OT, bool GELU>
 bool launch_typed(const LinearArgs& a, cudaStream_t s) {
-  // A few rows: dp4a on streamed weights until its multiplications (about a
-  // quarter of what a tensor core's tile start costs per 2^24) outweigh that.
-  // us for 8 rows: 512->512 2.7 against 4.8, 2050->5003 10.1 against 7.2; for 4:
-  // 4096->4096 5.8 against 8.1, 8192->8192 19 against 16.5; one row is always
-  // quicker, 8192->8192 13.6 against 16.3.
-  if (a.rows == 1 || (a.rows <= 8 && a.rows * a.n * a.k <= 1ll << 26)) {
+  // A few rows: dp4a on streamed weights until its multiplications outweigh a
+  // tensor core tile's start. us for 8 rows: 512->512 2.6 against 3.8,
+  // 4096->4096 9.8 against 7.0; for 4: 4096->4096 5.9 against 7.0, 8192->8192 19
+  // against 15.0; for one 4096->4096 3.6 against 8.2.
+  if (a.rows <= 8 && a.rows * a.n * a.k <= 1ll << 26) {
     if (a.rows == 1) launch_gemv<1, 4, OT, GELU>(a, s);
     else if (a.rows == 2) launch_gemv<2, 4, OT, GELU>(a, s);
     else if (a.rows <= 4) launch_gemv<4, 4, OT, GELU>(a, s);
     else launch_gemv<8, 2, OT, GELU>(a, s);
     return true;
   }
-  // k split over a cluster pays where k is long (17 rows, 2048->512: 5.8 us
-  // against 8.0 by tiles; 512->512 5.1 against 4.7) and, past 64 rows, where
-  // tiles would leave most SMs idle (128 rows, 2048->512: 7.6 against 8.2;
-  // 4096->4096 13.5 against 12.6)
+  // k split over a cluster pays where k is long (17 rows, 2048->512: 4.5 us
+  // against 8.0 by tiles; 512->512 5.1 against 3.8) and, past 64 rows, where
+  // tiles would leave most SMs idle (128 rows, 2048->512: 6.4 against 8.2;
+  // 4096->4096 13.5 against 11.7)
   if (a.k > 1024 && (a.rows <= 64 || (a.rows <= 128 && a.n <= 1024))) {
     if (a.rows <= 16) return launch_few<16, 5, OT, GELU>(a, s);
     if (a.rows <= 32) return launch_few<32, 5, OT, GELU>(a, s);

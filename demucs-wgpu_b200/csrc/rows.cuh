@@ -16,7 +16,9 @@
 // up to 16384 columns to a block; longer rows are re-read (from L2) for each
 // reduction. 16-bit rows are held as they lie and unpacked in every pass: one
 // more instruction per value and pass, half the registers, and so twice the
-// rows in flight.
+// rows in flight. Measured: norm 60000 x 1024 f32 78 us (6330 GB/s), 112896 x
+// 512 f32 -> bf16 62 us (5610), 112896 x 512 bf16 56 us (4120: by issue slots);
+// quantise 112896 x 2048 bf16 145 us (4790); norm of 1 x 512 1.8 us.
 #pragma once
 
 #include <algorithm>
@@ -41,7 +43,7 @@ DMX_DEVICE float max3_abs(float a, float b, float c) {
 // scale's significand is all ones or the remainder underflows; rows with such
 // a scale divide. Every value goes this way: ties are no rarity among 16-bit
 // inputs, whose quotients have few digits, and a branch for values near one
-// took most pieces (112896 x 2048 bf16: 235 us against 165). The integer is
+// took most pieces (112896 x 2048 bf16: 235 us against 145). The integer is
 // read off the sum with 1.5 * 2^23, whose last place is 1; the conversion
 // instructions share the special-function unit, which two of them per value
 // kept busy for longer than the row's memory traffic (316 us).

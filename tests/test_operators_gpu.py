@@ -619,7 +619,7 @@ LINEAR_SHAPES = [(1, 1, 1), (1, 3, 15), (1, 64, 16), (1, 512, 512), (1, 1000, 40
                  (100, 1000, 4000), (127, 127, 127), (128, 128, 128), (129, 257, 385), (192, 2048, 96),
                  (255, 33, 2049), (256, 512, 48), (257, 65, 512), (300, 2050, 700), (500, 48, 100),
                  (672, 1536, 512), (1000, 1, 77), (1345, 513, 511), (2688, 512, 2048), (4000, 17, 130),
-                 (5000, 1031, 24), (20001, 136, 200)]
+                 (5000, 1031, 24), (20001, 136, 200), (19001, 2055, 150)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEAR_SHAPES)
@@ -633,7 +633,7 @@ def test_quantized_linear_matches_64_bits(ops, m, n, k, ot):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 520, 700), (5, 130, 512), (12, 100, 96), (40, 257, 300), (90, 640, 2048),
-                                   (200, 384, 130), (700, 1025, 512)])
+                                   (200, 384, 130), (700, 1025, 512), (19008, 2056, 96)])
 @pytest.mark.parametrize("ot", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("act", [0, 1])
 @pytest.mark.parametrize("res,pad", [(False, 5), (True, 0), (True, 8)])
