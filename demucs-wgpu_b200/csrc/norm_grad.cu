@@ -95,7 +95,7 @@ void launch_norm_grad(const NormGradArgs& args, cudaStream_t s) {
         {launch_norm_grad_bf16_f32, launch_norm_grad_bf16_f16, launch_norm_grad_bf16_bf16}};
     launch[a.x_type][a.dy_type](a, parts, how, how == BY_SHIFT ? vec == VEC_32 : wide, s);
   }
-  if (sums)
+  if (sums && !(parts == 1 && a.cols <= 1024))
     launch_chained(norm_grad_join_kernel, (a.cols + 31) / 32, 1024, 0, s, true, 1, a.partials, parts, a.cols,
                    a.dweight, a.dbias);
 }

@@ -158,10 +158,12 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
   }
   if (!a.partials) return;
   // the block's row groups added in their order
-  const int pitch = grad_pitch(a.cols);
-  float* out = a.partials + (int64_t)blockIdx.x * 2 * pitch;
+  float* out = a.partials + (int64_t)blockIdx.x * 2 * grad_pitch(a.cols);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
+    // one block's sums are the gradients themselves
+    float* to = gridDim.x > 1 ? out + half * grad_pitch(a.cols) : half ? a.dbias : a.dweight;
+    if (!to) continue;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
       float t = 0.f;
 #pragma unroll
       for (int g = 0; g < per; ++g) t += sums[g][c];
-      out[half * pitch + c] = t;
+      to[c] = t;
     }
   }
 }

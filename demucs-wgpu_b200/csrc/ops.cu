@@ -51,7 +51,7 @@ struct OnDevice {
 
 // Largest row count, row length and pitch taken: offsets stay far inside 64 bits.
 constexpr int64_t kMaxRows = INT32_MAX, kMaxCols = INT32_MAX / 4, kMaxPitch = 1ll << 31;
-// 127 * 128 * k must stay below 2^31 for every pair of int8 rows, -128 included
+// 128 * 128 * k must stay below 2^31
 constexpr int64_t kMaxInner = 131071;
 
 [[noreturn]] void refuse(const char* what, const std::string& why) {

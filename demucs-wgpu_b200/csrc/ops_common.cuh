@@ -23,18 +23,6 @@ DMX_DEVICE __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 DMX_DEVICE __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// One element of an array whose type is known only at run time (uniform over the launch).
-DMX_DEVICE float load_as_f32(const void* p, int type, int64_t i) {
-  if (type == DMX_TYPE_F32) return static_cast<const float*>(p)[i];
-  if (type == DMX_TYPE_F16) return to_f32(static_cast<const __half*>(p)[i]);
-  return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-DMX_DEVICE void store_from_f32(void* p, int type, int64_t i, float v) {
-  if (type == DMX_TYPE_F32) static_cast<float*>(p)[i] = v;
-  else if (type == DMX_TYPE_F16) static_cast<__half*>(p)[i] = from_f32<__half>(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
-}
-
 // 16- and 32-byte accesses in inline PTX, so that a branch on a type known
 // only at run time stays a branch: the compiler would otherwise run all three
 // types' loads and conversions under predicates (twice the instructions of a
