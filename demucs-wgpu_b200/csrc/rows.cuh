@@ -134,13 +134,8 @@ struct RowSum<0> {
 // Piece j's values past the row's end become 0.
 template <bool VEC>
 DMX_DEVICE void mask8(const Pieces<VEC>& p, int j, float* v) {
-  if (VEC && !p.has(j, 0)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  } else if (p.ragged()) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = p.has(j, e) ? v[e] : 0.f;
-  }
+  for (int e = 0; e < 8; ++e) v[e] = p.has(j, e) ? v[e] : 0.f;
 }
 
 constexpr int kRowsThreads = 256;
@@ -214,12 +209,16 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
   for (int j = 0; j < NV; ++j) {
     get(j, v);
     centre8(v, mean);
-    mask8(p, j, v);
+    if (p.ragged()) mask8(p, j, v);
+    float2 t = s;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const float2 d = make_float2(v[e], v[e + 1]);
-      s = __ffma2_rn(d, d, s);
+      t = __ffma2_rn(d, d, t);
     }
+    // a piece past the row's end holds -mean: left out whole, as cheaper than masked
+    const bool in = p.has(j, 0);
+    s = make_float2(in ? t.x : s.x, in ? t.y : s.y);
   }
   const float rstd = 1.f / sqrtf(over.sum(s.x + s.y, sh[1]) / (float)a.cols + a.eps);
   if (p.t == 0 && live) {
@@ -273,9 +272,11 @@ DMX_DEVICE void row_in_registers(const RowArgs& a, int64_t row, bool live, const
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     value(j, y[j]);
-    mask8(p, j, y[j]);
+    if (p.ragged()) mask8(p, j, y[j]);
+    float t = top;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) top = max3_abs(top, y[j][e], y[j][e + 1]);
+    for (int e = 0; e < 8; e += 2) t = max3_abs(t, y[j][e], y[j][e + 1]);
+    top = p.has(j, 0) ? t : top;
   }
   const Quantizer quant(over.max(__float_as_uint(top), reinterpret_cast<uint32_t*>(sh[2])));
   if (!live) return;
