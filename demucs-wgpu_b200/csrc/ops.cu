@@ -8,6 +8,7 @@
 #include <cmath>
 #include <thread>
 
+#include "kernels.h"
 #include "ops.h"
 #include "runtime.cuh"
 
@@ -204,8 +205,22 @@ dmx_status dmx_ops_check(dmx_ops* ops, void* stream) {
     if (code == 0) return;
     CK(cudaMemsetAsync(ops->err, 0, sizeof(int), s));
     CK(cudaStreamSynchronize(s));
-    throw Error(DMX_ERR_TIMEOUT, "dmx_quantized_linear: a bounded wait gave up (code " +
-                                     std::to_string(code) + "); its outputs are not valid");
+    throw Error(DMX_ERR_TIMEOUT,
+                std::string(code == kSelftestCode ? "the self-test kernel" : "dmx_quantized_linear") +
+                    ": a bounded wait gave up (code " + std::to_string(code) +
+                    "); the outputs of dmx_quantized_linear since the last check are not valid");
+  });
+}
+
+dmx_status dmx_ops_selftest_wait_timeout(dmx_ops* ops, int wait_ms, void* stream) {
+  return guarded([&] {
+    const char* what = "dmx_ops_selftest_wait_timeout";
+    if (!ops) refuse(what, "ops is null");
+    if (wait_ms < 1 || wait_ms > 5000) refuse(what, "wait_ms must be in [1, 5000]");
+    OnDevice on(ops->device);
+    launch_selftest_wait((uint64_t)wait_ms * 1000000ull, kSelftestCode, ops->err,
+                         static_cast<cudaStream_t>(stream));
+    CK(cudaGetLastError());
   });
 }
 

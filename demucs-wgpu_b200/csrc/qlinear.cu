@@ -215,14 +215,11 @@ struct Pipe {
   uint64_t *full, *empty;
 };
 
-// After a wait gave up: nothing this CTA started may still write its shared
-// memory or read it when it exits. Waits (bounded) for the loads issued last
-// into each stage.
-template <int STAGES>
-DMX_DEVICE void drain_loads(const Pipe& p, uint32_t issued, int* err) {
-  for (uint32_t it = issued > STAGES ? issued - STAGES : 0; it < issued; ++it)
-    mbar_wait(&p.full[it % STAGES], (it / STAGES) & 1, err, 14);
-}
+// What a kernel's warps leave for its end: whether a wait gave up, and how many
+// stages each CTA began to load (a pair's: at the first, where they count).
+struct Ending {
+  uint32_t gave_up, issued[2];
+};
 // A barrier of both CTAs of a pair gets an arrival once the pair's MMAs so far are done.
 DMX_DEVICE void umma_commit_pair(uint64_t* bar) {
   asm volatile(
@@ -236,17 +233,14 @@ DMX_DEVICE void commit(uint64_t* bar) {
   if (PAIR) umma_commit_pair(bar);
   else umma_commit(bar);
 }
-// As drain_loads, for the MMAs issued so far.
-template <bool PAIR>
-DMX_DEVICE void drain_mmas(uint64_t* bar, int* err) {
-  commit<PAIR>(bar);
-  mbar_wait(bar, 0, err, 15);
-}
 // Shared memory of CTA `rank` of the cluster at this CTA's address p.
 DMX_DEVICE uint32_t of_rank(const void* p, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
+}
+DMX_DEVICE void st_cluster(uint32_t at, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 DMX_DEVICE int4 ld_cluster(uint32_t at) {
   int4 v;
@@ -305,6 +299,45 @@ DMX_DEVICE bool elect_one() {
 DMX_DEVICE bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
+// The same, a wait that gives up noted at every CTA that shares its loads and MMAs.
+template <bool PAIR>
+DMX_DEVICE bool noted_wait(uint64_t* bar, uint32_t parity, int* err, int code, Ending* end) {
+  if (warp_wait(bar, parity, err, code)) return true;
+  if (PAIR) {
+    st_cluster(of_rank(&end->gave_up, 0), 1);
+    st_cluster(of_rank(&end->gave_up, 1), 1);
+  } else {
+    *reinterpret_cast<volatile uint32_t*>(&end->gave_up) = 1;
+  }
+  return false;
+}
+// After a wait gave up, between two barriers of the CTAs that share its loads
+// and MMAs: what was begun is waited for, so that nothing writes shared memory,
+// or reads it or tensor memory, once they are another kernel's. These waits are
+// bounded too, but look past the raised flag, which is no reason to leave now.
+// For the CTA that issues the MMAs, whose elected lane of warp 1 did.
+template <int STAGES, bool PAIR>
+DMX_DEVICE void settle(const Pipe& pipe, const Ending& end, uint64_t* drain, uint32_t stage_bytes,
+                       bool elected) {
+  if (threadIdx.x < 32) {
+    const uint32_t mine = end.issued[0], other = PAIR ? end.issued[1] : mine, last = max(mine, other);
+    for (uint32_t it = last > STAGES ? last - STAGES : 0; it < last; ++it) {
+      uint64_t* bar = &pipe.full[it % STAGES];
+      if (elected) {
+        if (it >= mine) mbar_expect_tx(bar, stage_bytes);  // only the other CTA's bytes come
+        if (it >= other)                                   // its bytes never come
+          asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                       "r"(stage_bytes)
+                       : "memory");
+      }
+      __syncwarp();
+      mbar_wait(bar, (it / STAGES) & 1, nullptr, 0);
+    }
+  } else if (threadIdx.x < 64 && elected) {
+    commit<PAIR>(drain);
+    mbar_wait(drain, 0, nullptr, 0);
+  }
+}
 DMX_DEVICE void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 DMX_DEVICE void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -361,6 +394,7 @@ __global__ void __launch_bounds__(kFewThreads)
   uint64_t* done = pipe.empty + STAGES;
   uint64_t* drain = done + 1;
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  Ending* end = reinterpret_cast<Ending*>(slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int split = blockIdx.x % splits, n0 = (blockIdx.x / splits) * 128, m0 = blockIdx.y * BT;
@@ -375,6 +409,7 @@ __global__ void __launch_bounds__(kFewThreads)
     }
     mbar_init(done, 1);
     mbar_init(drain, 1);
+    *end = {};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc<false>(slot, S::COLS);
@@ -393,7 +428,7 @@ __global__ void __launch_bounds__(kFewThreads)
     uint32_t it = 0;
     for (int kb = lo; kb < hi; ++kb, ++it) {
       const uint32_t s = it % STAGES;
-      if (!warp_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 11)) break;
+      if (!noted_wait<false>(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 11, end)) break;
       if (elected) {
         unsigned char* dst = smem + s * S::STAGE;
         mbar_expect_tx(&pipe.full[s], S::STAGE);
@@ -401,12 +436,12 @@ __global__ void __launch_bounds__(kFewThreads)
         tma_load_2d(dst + S::A, &tm_x, &pipe.full[s], kb * kBlockK, m0);
       }
     }
-    if (it < count) drain_loads<STAGES>(pipe, it, a.err);
+    if (elected) end->issued[0] = it;
   } else if (warp == 1) {
     uint32_t it = 0;
     for (int kb = lo; kb < hi; ++kb, ++it) {
       const uint32_t s = it % STAGES;
-      if (!warp_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 12)) break;
+      if (!noted_wait<false>(&pipe.full[s], (it / STAGES) & 1, a.err, 12, end)) break;
       tc_after_sync();
       if (elected) {
         const uint32_t addr = smem_u32(smem + s * S::STAGE);
@@ -414,17 +449,14 @@ __global__ void __launch_bounds__(kFewThreads)
         umma_commit(&pipe.empty[s]);
       }
     }
-    if (elected) {
-      if (it < count) drain_mmas<false>(drain, a.err);
-      else umma_commit(done);
-    }
+    if (elected && it == count) umma_commit(done);
   }
   __syncwarp();
   int* part = reinterpret_cast<int*>(smem);  // [BT][128]
   if (warp >= 2 && warp < 6) {
     // lane = channel, column = row of x: [row][channel] is written without bank conflicts
     const int q = warp % 4;
-    const bool ok = warp_wait(done, 0, a.err, 13);
+    const bool ok = noted_wait<false>(done, 0, a.err, 13, end);
     tc_after_sync();
     const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
     if (ok) {
@@ -441,6 +473,7 @@ __global__ void __launch_bounds__(kFewThreads)
   }
   if (splits > 1) cluster_sync();
   else __syncthreads();
+  if (end->gave_up) settle<STAGES, false>(pipe, *end, drain, S::STAGE, elected);
   // each CTA of the cluster finishes its share of the rows, a warp a row and a
   // lane four channels of it
   const int rows = (int)min((int64_t)BT, a.rows - m0), n = n0 + 4 * lane;
@@ -679,6 +712,7 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
   uint64_t* acc_empty = acc_full + 2;        // [2]
   uint64_t* drain = acc_empty + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  Ending* end = reinterpret_cast<Ending*>(slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = PAIR ? blockIdx.x % 2 : 0;  // in the pair; the first issues its MMAs
@@ -693,6 +727,7 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
       mbar_init(&acc_empty[i], kCtas * S::EPI_WARPS);
     }
     mbar_init(drain, 1);
+    *end = {};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc<PAIR>(slot, S::COLS);
@@ -718,7 +753,7 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
       const int m0 = (int)(mt * S::ROWS + rank * 128), n0 = (int)(nt * BN + rank * 128);
       for (int kb = 0; kb < blocks; ++kb, ++it) {
         const uint32_t s = it % STAGES;
-        ok = warp_wait(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 21);
+        ok = noted_wait<PAIR>(&pipe.empty[s], ((it / STAGES) & 1) ^ 1, a.err, 21, end);
         if (!ok) break;
         if (elected) {
           unsigned char* dst = smem + s * S::STAGE;
@@ -735,20 +770,23 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
         }
       }
     }
-    if (!ok && rank == 0) drain_loads<STAGES>(pipe, it, a.err);
+    if (elected) {
+      if (PAIR) st_cluster(of_rank(&end->issued[rank], 0), it);
+      else end->issued[0] = it;
+    }
   } else if (warp == 1) {
     uint32_t it = 0;
     int tl = 0;
     bool ok = true;
     for (uint32_t t = begin; t < order.total && ok && rank == 0; t += step, ++tl) {
       const int acc = tl & 1;
-      ok = warp_wait(&acc_empty[acc], ((tl >> 1) & 1) ^ 1, a.err, 22);
+      ok = noted_wait<PAIR>(&acc_empty[acc], ((tl >> 1) & 1) ^ 1, a.err, 22, end);
       if (!ok) break;
       tc_after_sync();
       const uint32_t d = tmem + (uint32_t)(acc * BN);
       for (int kb = 0; kb < blocks; ++kb, ++it) {
         const uint32_t s = it % STAGES;
-        ok = warp_wait(&pipe.full[s], (it / STAGES) & 1, a.err, 23);
+        ok = noted_wait<PAIR>(&pipe.full[s], (it / STAGES) & 1, a.err, 23, end);
         if (!ok) break;
         tc_after_sync();
         if (elected) {
@@ -759,7 +797,6 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
       }
       if (ok && elected) commit<PAIR>(&acc_full[acc]);
     }
-    if (!ok && elected) drain_mmas<PAIR>(drain, a.err);
   } else {
     // this warp: rows 32 quarter + lane, columns c_lo .. c_lo + WIDTH - 1 of each tile
     constexpr int WIDTH = S::WIDTH;
@@ -810,7 +847,7 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
       if (2 * lane < WIDTH) col[lane] = sb;
       __syncwarp();
       if (t + step < order.total) fetch(t + step);
-      ok = ok && warp_wait(&acc_full[acc], (tl >> 1) & 1, a.err, 24);
+      ok = ok && noted_wait<PAIR>(&acc_full[acc], (tl >> 1) & 1, a.err, 24, end);
       tc_after_sync();
       if (ok && n0 < a.n)
         tile_share<WIDTH, OT, GELU>(a, lines, from + (uint32_t)(acc * BN), col, row_scale, m0, n0,
@@ -829,6 +866,11 @@ __global__ void __launch_bounds__(Tile<BN>::THREADS, 1)
   // a pair's MMAs read both CTAs' memory, and its barriers are the first's
   if (PAIR) cluster_sync();
   else __syncthreads();
+  if (end->gave_up) {
+    if (rank == 0) settle<STAGES, PAIR>(pipe, *end, drain, S::STAGE, elected);
+    if (PAIR) cluster_sync();
+    else __syncthreads();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_after_sync();

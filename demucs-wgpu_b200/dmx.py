@@ -32,7 +32,7 @@ EXPORTS = (
     "dmx_set_stage_timing", "dmx_stage_times", "dmx_kernel_launches", "dmx_stream",
     "dmx_synchronize", "dmx_read_tensor", "dmx_shift_offsets", "dmx_ipc_export", "dmx_ipc_open",
     "dmx_ipc_close", "dmx_rows_copy", "dmx_rows_add", "dmx_separate_track_windowed",
-    "dmx_ops_create", "dmx_ops_destroy", "dmx_ops_check", "dmx_layer_norm",
+    "dmx_ops_create", "dmx_ops_destroy", "dmx_ops_check", "dmx_ops_selftest_wait_timeout", "dmx_layer_norm",
     "dmx_layer_norm_backward_workspace", "dmx_layer_norm_backward", "dmx_quantize_rows",
     "dmx_layer_norm_quantize", "dmx_quantized_linear",
 )
@@ -168,6 +168,7 @@ def lib():
         L.dmx_ops_destroy.argtypes = [vp]
         L.dmx_ops_destroy.restype = None
         L.dmx_ops_check.argtypes = [vp, vp]
+        L.dmx_ops_selftest_wait_timeout.argtypes = [vp, ci, vp]
         for name in ("dmx_layer_norm", "dmx_layer_norm_backward", "dmx_quantize_rows",
                      "dmx_layer_norm_quantize", "dmx_quantized_linear"):
             getattr(L, name).argtypes = [vp, ctypes.c_char_p, vp]
@@ -527,6 +528,11 @@ class Ops:
     def check(self, stream: int = 0):
         """Waits for ``stream``; raises DmxError code 4 if a wait in a kernel gave up."""
         _check(self._L.dmx_ops_check(self._h, stream))
+
+    def selftest_wait_timeout(self, wait_ms: int = 200, stream: int = 0):
+        """Enqueues a wait that gives up after ``wait_ms`` and raises the context's
+        flag: the next check raises DmxError code 4."""
+        _check(self._L.dmx_ops_selftest_wait_timeout(self._h, wait_ms, stream))
 
     def layer_norm(self, x: int, x_type: int, rows: int, cols: int, y: int, y_type: int,
                    weight: int = 0, bias: int = 0, param_type: int = TYPE_F32, eps: float = 1e-5,

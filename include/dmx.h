@@ -444,6 +444,12 @@ void dmx_ops_destroy(dmx_ops* ops);
 /* Waits (bounded) until `stream` has drained; DMX_ERR_TIMEOUT if a wait inside
  * a kernel of this context gave up since the last check (the flag is cleared). */
 dmx_status dmx_ops_check(dmx_ops* ops, void* stream);
+/* Self-test of that path, as dmx_selftest_wait_timeout: enqueues one warp that
+ * waits on a device flag that nothing sets, gives up after `wait_ms` (1..5000)
+ * and raises the context's flag. Calls enqueued behind it see the flag, give up
+ * at once and end; the next dmx_ops_check returns DMX_ERR_TIMEOUT and leaves
+ * the context usable. */
+dmx_status dmx_ops_selftest_wait_timeout(dmx_ops* ops, int wait_ms, void* stream);
 
 /* Layer norm of every row: y = (x - mean) rstd weight + bias with
  * mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps).

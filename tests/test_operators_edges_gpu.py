@@ -1,0 +1,56 @@
+"""The operators (GPU) where calls meet limits: waits that give up, buffers that
+end with their last value, operands of different alignment, workspaces of
+other calls. The plain implementations and bounds are test_operators_gpu.py's.
+"""
+
+import pytest
+
+from test_operators_gpu import _linear_inputs, _linear_want, _product, _run_linear, _within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import dmx
+
+    o = dmx.Ops(0)
+    yield o
+    o.check()
+    o.close()
+
+
+# --- waits that give up -------------------------------------------------------
+
+# every kernel with waits: k split over a cluster and not, tiles of one CTA and
+# of a pair, one round of tiles and many, one stage of k and many
+@pytest.mark.parametrize("m,n,k", [(17, 130, 1100), (20, 300, 2050), (100, 512, 8192), (12, 64, 48), (300, 128, 512),
+                                   (700, 2055, 1000), (20001, 40, 200), (8192, 4096, 2048), (9001, 2050, 130)])
+def test_calls_behind_a_raised_flag_end_and_the_next_ones_are_right(ops, m, n, k):
+    import dmx
+    import torch
+
+    x, w, xs, ws, b = _linear_inputs(m, n, k, m + k)
+    want, bound = _linear_want(_product(x, w, k), xs, ws, b, 0, None, "f32")
+    first = _run_linear(ops, x, w, k, "f32", xs, ws, b).clone()
+    _within(first, want, bound, "before")
+    for _ in range(3):
+        ops.selftest_wait_timeout(20)
+        for _ in range(4):
+            _run_linear(ops, x, w, k, "f32", xs, ws, b)
+        with pytest.raises(dmx.DmxError, match="self-test kernel: a bounded wait gave up") as e:
+            ops.check()
+        assert e.value.code == 4
+        ops.check()  # reported once
+        assert torch.equal(_run_linear(ops, x, w, k, "f32", xs, ws, b), first)
+        ops.check()
+
+
+def test_the_self_test_of_a_wait_refuses_other_limits(ops):
+    import dmx
+
+    for ms in (0, -1, 5001):
+        with pytest.raises(dmx.DmxError, match="wait_ms") as e:
+            ops.selftest_wait_timeout(ms)
+        assert e.value.code == 1
+    ops.check()
