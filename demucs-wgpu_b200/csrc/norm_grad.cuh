@@ -180,9 +180,11 @@ __global__ void __launch_bounds__(kGradThreads, NV == 4 ? 1 : 2)
   }
 }
 
-// `bytes` (0..16, the rest as zeros) of 16 from global to this thread's shared memory.
+// `bytes` (0..16, the rest as zeros) of 16 from global to this thread's shared
+// memory. With a clobber: what lay there before is read by plain loads, which
+// the compiler could otherwise move below the copy that overwrites it.
 DMX_DEVICE void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // Rows of up to blockDim.x * 16 columns, a group of blockDim.x threads each, R

@@ -5,7 +5,8 @@ other calls. The plain implementations and bounds are test_operators_gpu.py's.
 
 import pytest
 
-from test_operators_gpu import _linear_inputs, _linear_want, _product, _run_linear, _within
+from test_operators_gpu import (HALF_ULP, TINY, _back64, _back_inputs, _linear_inputs, _linear_want, _padded, _product,
+                                _run_back, _run_linear, _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,21 @@ def test_the_self_test_of_a_wait_refuses_other_limits(ops):
             ops.selftest_wait_timeout(ms)
         assert e.value.code == 1
     ops.check()
+
+
+# --- rows copied ahead --------------------------------------------------------
+
+# many rows to each group of threads, so that every stage of its ring of copies
+# is read and filled again, at each depth of the ring and one or two rows at a time
+@pytest.mark.parametrize("rows,cols,pad", [(5003, 1032, 0), (4001, 2048, 0), (2611, 4099, 5), (1999, 8195, 5),
+                                           (1501, 10248, 0), (1207, 12288, 0), (1103, 16384, 0)])
+@pytest.mark.parametrize("xt,dyt", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f32")])
+def test_backward_of_many_long_rows(ops, rows, cols, pad, xt, dyt):
+    dy, x, w, mean, rstd = _back_inputs(rows, cols, xt, dyt, rows + cols)
+    _, dyv = _padded(dy, dy.dtype, pad)
+    _, xv = _padded(x, x.dtype, pad)
+    dx, dw, db = _run_back(ops, dyv, xv, w, mean, rstd, pad=pad)
+    dx64, dw64, db64, e_dx, e_w, e_b = _back64(dy, x, w, mean, rstd)
+    _within(dx, dx64, e_dx + HALF_ULP[xt] * (dx64.abs() + e_dx) + TINY[xt], "dx")
+    _within(dw, dw64, e_w, "dweight")
+    _within(db, db64, e_b, "dbias")
