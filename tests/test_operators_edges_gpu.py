@@ -73,3 +73,24 @@ def test_backward_of_many_long_rows(ops, rows, cols, pad, xt, dyt):
     _within(dx, dx64, e_dx + HALF_ULP[xt] * (dx64.abs() + e_dx) + TINY[xt], "dx")
     _within(dw, dw64, e_w, "dweight")
     _within(db, db64, e_b, "dbias")
+
+
+# --- buffers that end with their last value -----------------------------------
+
+@pytest.mark.parametrize("k", [1, 3, 15, 17, 100, 509, 1031, 2050, 4097])
+@pytest.mark.parametrize("m,n", [(1, 7), (2, 64), (4, 1001), (8, 130), (20, 96), (300, 33)])
+def test_quantized_linear_of_buffers_that_end_with_the_last_row(ops, m, n, k):
+    import torch
+
+    x, w, xs, ws, b = _linear_inputs(m, n, k, m + n + k)
+    ld = x.shape[1]
+
+    def cut(t):  # the same rows, the last one without its padding
+        flat = torch.empty((t.shape[0] - 1) * ld + k, dtype=torch.int8, device="cuda")
+        rows = flat.as_strided((t.shape[0], k), (ld, 1))
+        rows.copy_(t[:, :k])
+        return rows
+
+    got = _run_linear(ops, cut(x), cut(w), k, "f32", xs, ws, b)
+    want, bound = _linear_want(_product(x, w, k), xs, ws, b, 0, None, "f32")
+    _within(got, want, bound, "out")
