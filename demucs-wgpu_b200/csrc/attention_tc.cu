@@ -490,12 +490,12 @@ bool launch_attention_tc(const float* q, int ldq, int q_col, const float* kv, in
   p.scale = scale;
   p.err = err;
   static PerDevice attr;
-  if (attr.first()) {
+  attr.once([] {
     cudaFuncSetAttribute(attention_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          AttnSmem<false>::TOTAL);
     cudaFuncSetAttribute(attention_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          AttnSmem<true>::TOTAL);
-  }
+  });
   const dim3 grid((nq + QT - 1) / QT, heads, B);
   if (bf16_in)
     attention_tc_kernel<true><<<grid, 192, AttnSmem<true>::TOTAL, s>>>(mkv, mv, mq, p);

@@ -13,14 +13,18 @@ namespace dmx {
 // Once per device for per-context settings such as a kernel's dynamic
 // shared-memory limit: a function attribute belongs to the context of the
 // device that was current when it was set, so each GPU a process launches on
-// needs its own. `first()` is true the first time it is asked on a device.
+// needs its own. once() returns when the settings are made: threads that get
+// there together each make them (the same again), so that none launches before.
 struct PerDevice {
   std::atomic<uint64_t> done{0};
-  bool first() {
+  template <typename F>
+  void once(F&& set) {
     int d = 0;
     cudaGetDevice(&d);
     const uint64_t bit = 1ull << (d & 63);
-    return (done.fetch_or(bit) & bit) == 0;
+    if (done.load(std::memory_order_acquire) & bit) return;
+    set();
+    done.fetch_or(bit, std::memory_order_release);
   }
 };
 

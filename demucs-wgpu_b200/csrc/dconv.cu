@@ -499,12 +499,12 @@ template <int C>
 void launch_c(const DConvArgs& a, cudaStream_t s) {
   using M = Smem<C>;
   static PerDevice configured;
-  if (configured.first()) {
+  configured.once([] {
     set_smem(dconv_row_kernel<C>, M::kRow);
     set_smem(dconv_conv1_kernel<C>, M::kConv1);
     set_smem(dconv_conv2_kernel<C, false>, M::kConv2);
     set_smem(dconv_conv2_kernel<C, true>, M::kConv2);
-  }
+  });
   if (a.T <= kTile) {
     dconv_row_kernel<C><<<a.rows, kThreads, M::kRow, s>>>(a);
     return;
@@ -521,7 +521,7 @@ void launch_zstats_c(const float* y, int ld, int rows, int T, const float* n1w, 
                      cudaStream_t s) {
   const size_t bytes = sizeof(float) * (Zq<C>::N + Zq<C>::ZL * 256);
   static PerDevice configured;
-  if (configured.first()) set_smem(dconv_zstats_kernel<C>, bytes);
+  configured.once([&] { set_smem(dconv_zstats_kernel<C>, bytes); });
   dconv_zstats_kernel<C><<<dim3(dconv_zstats_parts(T), rows), 256, bytes, s>>>(y, ld, T, n1w, n1b,
                                                                               st1, part, zq);
   launch_sum_partials(part, dconv_zstats_parts(T), rows, st2, s);

@@ -1343,12 +1343,12 @@ bool launch_c(const DConvArgs& a, cudaStream_t s) {
   for (int i = 0; i < S::HID; ++i) k.n1w[i] = *src++;
   for (int i = 0; i < S::HID; ++i) k.n1b[i] = *src++;
   static PerDevice configured;
-  if (configured.first()) {
+  configured.once([] {
     cudaFuncSetAttribute(dconv_tc_row_kernel<C, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          S::SMEM);
     cudaFuncSetAttribute(dconv_tc_row_kernel<C, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          S::SMEM);
-  }
+  });
   auto row_kernel = a.single ? dconv_tc_row_kernel<C, false> : dconv_tc_row_kernel<C, true>;
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -1401,9 +1401,10 @@ bool launch_wide(const DConvArgs& a, cudaStream_t s) {
   for (int i = 0; i < S::HID; ++i) k.n1w[i] = *src++;
   for (int i = 0; i < S::HID; ++i) k.n1b[i] = *src++;
   static PerDevice configured;
-  if (configured.first())
+  configured.once([] {
     cudaFuncSetAttribute(dconv_tc_wide_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          S::SMEM);
+  });
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -457,10 +457,11 @@ template <typename XT, typename DT, typename PT, int VEC, int THREADS, int R>
 void launch_norm_grad_block(const NormGradArgs& a, int parts, dim3 block, size_t smem, bool wide,
                             int ahead, cudaStream_t s) {
   auto kernel = norm_grad_block_kernel<XT, DT, PT, VEC, THREADS, R>;
-  static PerDevice once;
-  if (once.first())
+  static PerDevice configured;
+  configured.once([&] {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          (VEC == BY_SHIFT ? 128 : 220) * 1024);
+  });
   launch_chained(kernel, parts, block, smem, s, true, 1, a, wide, ahead);
 }
 

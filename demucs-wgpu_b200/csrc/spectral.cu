@@ -401,9 +401,10 @@ void launch_istft(const float* spec, const float4* norm, const float* window, co
                   const float* envelope, const float* time_branch, const float4* norm_t, float* out,
                   int B, cudaStream_t s) {
   static PerDevice configured;
-  if (configured.first())
+  configured.once([] {
     cudaFuncSetAttribute(istft_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          (int)kIstftSmem);
+  });
   // hops 3 .. 339 of the centred signal hold the segment's samples
   const int groups = (337 + kIstftHops - 1) / kIstftHops;
   istft_kernel<<<dim3(4, groups, B), kIstftThreads, kIstftSmem, s>>>(spec, norm, window, tw,

@@ -708,9 +708,10 @@ void launch_cfg(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap&
 #define DMX_TC_CASE(E)                                                                        \
   case E: {                                                                                   \
     static PerDevice attr;                                                                    \
-    if (attr.first())                                                                         \
+    attr.once([] {                                                                            \
       cudaFuncSetAttribute(tc_gemm_kernel<BN, BK, STAGES, E, MODE, RB>,                      \
                            cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);          \
+    });                                                                                       \
     tc_gemm_kernel<BN, BK, STAGES, E, MODE, RB><<<grid, kThreads, smem, s>>>(ma, mb, mblo, p); \
     break;                                                                                    \
   }

@@ -243,9 +243,10 @@ void launch_flash_attention(const float* q, int ldq, const float* k, const float
                             cudaStream_t s) {
   const size_t smem = sizeof(float) * (AD * (AQ + 4) + AD * (AK + 4) + AK * AD + AK * (AQ + 4));
   static PerDevice configured;
-  if (configured.first())
+  configured.once([&] {
     cudaFuncSetAttribute(flash_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          (int)smem);
+  });
   flash_attention_kernel<<<dim3((nq + AQ - 1) / AQ, heads, B), 256, smem, s>>>(
       q, ldq, k, v, ldkv, o, ldo, nq, nk, scale);
 }

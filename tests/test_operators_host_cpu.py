@@ -41,3 +41,35 @@ int main() {
     r = _run(tmp_path, "tail.cpp", source, ["g++", "-std=c++17", "-O1", "-fno-strict-aliasing",
                                             "-fsanitize=address"])
     assert r.returncode == 0 and r.stdout == "ok\n", r.stderr[:2000]
+
+
+def test_settings_of_a_device_are_made_before_any_thread_goes_on(tmp_path):
+    # a second thread asks while the first is still making them, and a third afterwards
+    source = r"""
+#include <chrono>
+#include <cstdio>
+#include <thread>
+#include "common.cuh"
+int main() {
+  dmx::PerDevice configured;
+  std::atomic<int> begun{0}, made{0}, early{0};
+  auto set = [&] {
+    if (begun++ == 0) std::this_thread::sleep_for(std::chrono::milliseconds(300));
+    ++made;
+  };
+  std::thread first([&] { configured.once(set); });
+  while (begun == 0) std::this_thread::yield();
+  std::thread second([&] {
+    configured.once(set);
+    early = made == 0;
+  });
+  second.join();
+  first.join();
+  const int before = made;
+  configured.once(set);
+  std::printf("%d %d\n", early.load(), made - before);
+}
+"""
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    r = _run(tmp_path, "once.cu", source, [nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a"])
+    assert r.returncode == 0 and r.stdout == "0 0\n", (r.stdout, r.stderr[:2000])
