@@ -173,7 +173,7 @@ void launch_rows(bool add, float* dst, int64_t dld, const float* src, int64_t sl
 
 // selftest.cu — one warp waits on a device flag nothing sets and, after
 // limit_ns, stores `code` into err and returns (the bounded-wait error path).
-void launch_selftest_wait(uint64_t limit_ns, int code, int* err, cudaStream_t s);
+cudaError_t launch_selftest_wait(uint64_t limit_ns, int code, int* err, cudaStream_t s);
 
 // bag.cu — the bag's per-source weighted combination (api.rs:319-361).
 // For source s: out = (sum over j < count[s] of out[net[s][j]] * weight[s][j])

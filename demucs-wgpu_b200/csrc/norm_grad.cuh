@@ -459,8 +459,8 @@ void launch_norm_grad_block(const NormGradArgs& a, int parts, dim3 block, size_t
   auto kernel = norm_grad_block_kernel<XT, DT, PT, VEC, THREADS, R>;
   static PerDevice configured;
   configured.once([&] {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         (VEC == BY_SHIFT ? 128 : 220) * 1024);
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (VEC == BY_SHIFT ? 128 : 220) * 1024));
   });
   launch_chained(kernel, parts, block, smem, s, true, 1, a, wide, ahead);
 }

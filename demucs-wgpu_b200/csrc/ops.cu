@@ -34,6 +34,12 @@ int sm_count() {
   return n;
 }
 
+void check_cuda(cudaError_t e) {
+  if (e == cudaSuccess) return;
+  cudaGetLastError();
+  throw Error(DMX_ERR_CUDA, std::string("an operator's kernel could not be launched: ") + cudaGetErrorString(e));
+}
+
 }  // namespace dmx
 
 namespace {
@@ -218,9 +224,8 @@ dmx_status dmx_ops_selftest_wait_timeout(dmx_ops* ops, int wait_ms, void* stream
     if (!ops) refuse(what, "ops is null");
     if (wait_ms < 1 || wait_ms > 5000) refuse(what, "wait_ms must be in [1, 5000]");
     OnDevice on(ops->device);
-    launch_selftest_wait((uint64_t)wait_ms * 1000000ull, kSelftestCode, ops->err,
-                         static_cast<cudaStream_t>(stream));
-    CK(cudaGetLastError());
+    check_cuda(launch_selftest_wait((uint64_t)wait_ms * 1000000ull, kSelftestCode, ops->err,
+                                    static_cast<cudaStream_t>(stream)));
   });
 }
 
@@ -245,7 +250,6 @@ dmx_status dmx_layer_norm(dmx_ops* ops, const dmx_layer_norm_args* g, void* stre
     check_in_place(what, a.x, a.x_type, a.x_ld, a.y, a.y_type, a.y_ld);
     OnDevice on(ops->device);
     launch_rows(a, static_cast<cudaStream_t>(stream));
-    CK(cudaGetLastError());
   });
 }
 
@@ -302,7 +306,6 @@ dmx_status dmx_layer_norm_backward(dmx_ops* ops, const dmx_layer_norm_backward_a
     }
     OnDevice on(ops->device);
     launch_norm_grad(a, static_cast<cudaStream_t>(stream));
-    CK(cudaGetLastError());
   });
 }
 
@@ -321,7 +324,6 @@ dmx_status dmx_quantize_rows(dmx_ops* ops, const dmx_quantize_rows_args* g, void
     set_quantized(what, g, xb, &a);
     OnDevice on(ops->device);
     launch_rows(a, static_cast<cudaStream_t>(stream));
-    CK(cudaGetLastError());
   });
 }
 
@@ -338,7 +340,6 @@ dmx_status dmx_layer_norm_quantize(dmx_ops* ops, const dmx_layer_norm_quantize_a
     set_quantized(what, g, xb, &a);
     OnDevice on(ops->device);
     launch_rows(a, static_cast<cudaStream_t>(stream));
-    CK(cudaGetLastError());
   });
 }
 
@@ -388,7 +389,6 @@ dmx_status dmx_quantized_linear(dmx_ops* ops, const dmx_quantized_linear_args* g
     OnDevice on(ops->device);
     if (!launch_quantized_linear(a, static_cast<cudaStream_t>(stream)))
       throw Error(DMX_ERR_CUDA, "dmx_quantized_linear: a tensor map could not be encoded");
-    CK(cudaGetLastError());
   });
 }
 

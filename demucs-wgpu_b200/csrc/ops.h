@@ -11,6 +11,12 @@ namespace dmx {
 // SMs of the current device.
 int sm_count();
 
+// Throws (an Error that the entry points turn into a status) if a CUDA call of
+// an operator failed, and takes its error off the thread's last one. Statuses
+// are asked where they arise: the last error may be one that the caller's own
+// calls left, which is neither the operator's nor its to clear.
+void check_cuda(cudaError_t e);
+
 // One pass over rows: optionally the layer norm, then either a store (y) or
 // the 8-bit quantisation (q, scale).
 struct RowArgs {

@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "dmx.h"
+#include "ops.h"
 
 namespace dmx {
 
@@ -380,7 +381,7 @@ void launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cu
   cfg.stream = s;
   cfg.attrs = attrs;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
 }
 
 // The widest access that suits rows of `ld` elements of `bytes` bytes from p

@@ -921,8 +921,9 @@ bool launch_few(const LinearArgs& a, cudaStream_t s) {
   using S = FewSmem<BT, STAGES>;
   auto kernel = linear_few_kernel<BT, STAGES, OT, GELU>;
   static PerDevice configured;
-  configured.once(
-      [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL); });
+  configured.once([&] {
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+  });
   const int64_t tiles = (a.n + 127) / 128;
   const int mtiles = (int)((a.rows + BT - 1) / BT);
   const int blocks = (a.k + kBlockK - 1) / kBlockK;
@@ -943,8 +944,9 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
     return false;
   auto kernel = linear_tile_kernel<BN, OT, GELU>;
   static PerDevice configured;
-  configured.once(
-      [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL); });
+  configured.once([&] {
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+  });
   const int64_t mtiles = (a.rows + S::ROWS - 1) / S::ROWS, ntiles = (a.n + BN - 1) / BN;
   if (mtiles * ntiles > INT32_MAX) return false;  // no memory holds such an output
   const TileOrder order = {(uint32_t)mtiles, (uint32_t)ntiles, (uint32_t)(mtiles * ntiles)};

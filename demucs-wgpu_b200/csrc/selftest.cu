@@ -38,8 +38,12 @@ __global__ void selftest_wait_kernel(uint64_t limit_ns, int code, int* __restric
 
 }  // namespace
 
-void launch_selftest_wait(uint64_t limit_ns, int code, int* err, cudaStream_t s) {
-  selftest_wait_kernel<<<1, 32, 0, s>>>(limit_ns, code, err);
+cudaError_t launch_selftest_wait(uint64_t limit_ns, int code, int* err, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = 1;
+  cfg.blockDim = 32;
+  cfg.stream = s;
+  return cudaLaunchKernelEx(&cfg, selftest_wait_kernel, limit_ns, code, err);
 }
 
 }  // namespace dmx

@@ -94,3 +94,32 @@ def test_quantized_linear_of_buffers_that_end_with_the_last_row(ops, m, n, k):
     got = _run_linear(ops, cut(x), cut(w), k, "f32", xs, ws, b)
     want, bound = _linear_want(_product(x, w, k), xs, ws, b, 0, None, "f32")
     _within(got, want, bound, "out")
+
+
+# --- errors that are not the operators' ---------------------------------------
+
+def test_an_error_the_caller_left_is_neither_reported_nor_cleared(ops):
+    import ctypes
+
+    import torch
+
+    rt = ctypes.CDLL("libcudart.so.12")  # the one that the library and torch are linked to
+    x, y, dx = torch.randn(3, 40, 48, device="cuda")
+    mean, rstd, s = torch.ones(3, 40, device="cuda")
+    dw = torch.empty(48, device="cuda")
+    q, w = torch.zeros(2, 40, 48, dtype=torch.int8, device="cuda")
+    room = torch.empty(ops.layer_norm_backward_workspace(40, 48), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    p = torch.Tensor.data_ptr
+    calls = [lambda: ops.layer_norm(p(x), 0, 40, 48, p(y), 0),
+             lambda: ops.layer_norm_backward(p(y), 0, p(x), 0, p(mean), p(rstd), 40, 48, p(room), room.numel(),
+                                             dx=p(dx), dweight=p(dw)),
+             lambda: ops.quantize_rows(p(x), 0, 40, 48, p(q), p(s)),
+             lambda: ops.layer_norm_quantize(p(x), 0, 40, 48, p(q), p(s)),
+             lambda: ops.quantized_linear(p(q), p(w), p(y), 0, 40, 40, 48),
+             lambda: ops.quantized_linear(p(q), p(w), p(y), 0, 1, 40, 48)]
+    for call in calls:
+        assert rt.cudaSetDevice(100000) == 101  # cudaErrorInvalidDevice: a mistake of the caller's own
+        call()
+        assert rt.cudaGetLastError() == 101 and rt.cudaGetLastError() == 0
+    ops.check()
