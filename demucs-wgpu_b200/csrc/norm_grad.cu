@@ -30,12 +30,17 @@ int64_t most_parts(int64_t cols, bool vec) {
   return cols <= 1024 || cols > kGradBlockCols ? 296 : vec ? 148 : 444;
 }
 
-// As many of them as give each the same number of turns.
-int parts_of(int64_t rows, int64_t cols, bool vec) {
+// What a block takes in one turn, in units of which the rows make this many.
+int64_t units_of(int64_t rows, int64_t cols) {
   const int64_t each = cols <= 128 ? 32 : cols <= 256 ? 16 : cols <= 1024 ? 8
                        : cols <= kGradBlockCols ? grad_groups((int)cols) : 1;
+  return (rows + each - 1) / each;
+}
+
+// As many blocks as give each the same number of turns.
+int parts_of(int64_t rows, int64_t cols, bool vec) {
   const int64_t most = most_parts(cols, vec);
-  const int64_t units = (rows + each - 1) / each, turns = (units + most - 1) / most;
+  const int64_t units = units_of(rows, cols), turns = (units + most - 1) / most;
   return turns ? (int)((units + turns - 1) / turns) : 0;
 }
 
@@ -68,8 +73,9 @@ __global__ void __launch_bounds__(1024)
 
 }  // namespace
 
+// Enough for fewer rows too, which may take more blocks (of fewer turns each).
 size_t norm_grad_workspace(int64_t rows, int64_t cols) {
-  const int parts = std::max(parts_of(rows, cols, true), parts_of(rows, cols, false));
+  const int64_t parts = std::min(units_of(rows, cols), std::max(most_parts(cols, true), most_parts(cols, false)));
   return (size_t)parts * 2 * (size_t)grad_pitch((int)cols) * sizeof(float);
 }
 

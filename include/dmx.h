@@ -481,7 +481,8 @@ dmx_status dmx_layer_norm(dmx_ops* ops, const dmx_layer_norm_args* args, void* s
  * added to (rows 0: zeros). They are summed in a fixed order through
  * `workspace`, at least dmx_layer_norm_backward_workspace(rows, cols) bytes on
  * a 16-byte boundary, which the call overwrites and may be reused once the
- * stream has passed it; it may be NULL when neither is wanted. In place: dx
+ * stream has passed it; it may be NULL when neither is wanted. The size does
+ * not fall with more rows: a workspace serves every call of up to its rows. In place: dx
  * may be dy or x, with the same type and pitch. */
 size_t dmx_layer_norm_backward_workspace(int64_t rows, int64_t cols);
 typedef struct {

@@ -82,3 +82,14 @@ def test_packed_arguments_have_the_layout_of_the_structs(tmp_path):
             first = next(b for b in range(len(one)) if one[b])
             # an integer 1 is its lowest byte; the float 1 has its first set byte at offset + 2
             assert first == int(offset) + (2 if names.split()[i] == "eps" else 0), (name, names.split()[i])
+
+
+def test_backward_workspace_of_more_rows_serves_fewer():
+    size = dmx.lib().dmx_layer_norm_backward_workspace
+    for cols in (1, 64, 200, 512, 1000, 1031, 2048, 8195, 16384, 16385, 40000):
+        last = 0
+        for rows in range(1, 12000 if cols <= 512 else 5000):
+            got = size(rows, cols)
+            assert got >= last, (rows, cols)
+            last = got
+        assert size(10**6, cols) >= last and size(2**31 - 1, cols) == size(2**31 - 2, cols)

@@ -123,3 +123,30 @@ def test_an_error_the_caller_left_is_neither_reported_nor_cleared(ops):
         call()
         assert rt.cudaGetLastError() == 101 and rt.cudaGetLastError() == 0
     ops.check()
+
+
+# --- workspaces of other calls ------------------------------------------------
+
+@pytest.mark.parametrize("most,fewer,cols", [(2688, (2376, 2368, 2361, 17), 512), (4095, (444, 443, 297, 148, 3), 8195),
+                                             (6000, (4737, 4736, 300), 257), (3000, (1777, 1776, 740), 1500),
+                                             (700, (296, 148), 17000)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_backward_in_the_workspace_of_a_larger_call(ops, most, fewer, cols, shift):
+    # a training loop's workspace, made for its largest batch; rows on 16 bytes and off them
+    import torch
+
+    size = ops.layer_norm_backward_workspace(most, cols)
+    room = torch.full((size + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+    for rows in (most, *fewer):
+        dy, x, w, mean, rstd = _back_inputs(rows, cols, "bf16", "bf16", rows)
+        pad = (-cols) % 8 + shift
+        _, dyv = _padded(dy, dy.dtype, pad)
+        _, xv = _padded(x, x.dtype, pad)
+        want = _run_back(ops, dyv, xv, w, mean, rstd, pad=pad)
+        dx = torch.empty(rows, cols + pad, dtype=x.dtype, device="cuda")[:, :cols]
+        dw, db = torch.empty(2, cols, device="cuda")
+        ops.layer_norm_backward(dyv.data_ptr(), 2, xv.data_ptr(), 2, mean.data_ptr(), rstd.data_ptr(), rows, cols,
+                                room.data_ptr(), size, weight=w.data_ptr(), dx=dx.data_ptr(), dweight=dw.data_ptr(),
+                                dbias=db.data_ptr(), dy_ld=cols + pad, x_ld=cols + pad, dx_ld=cols + pad)
+        assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), want)), rows
+        assert (room[size:] == 0xAB).all(), "wrote past the workspace"
