@@ -150,3 +150,50 @@ def test_backward_in_the_workspace_of_a_larger_call(ops, most, fewer, cols, shif
                                 dbias=db.data_ptr(), dy_ld=cols + pad, x_ld=cols + pad, dx_ld=cols + pad)
         assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), want)), rows
         assert (room[size:] == 0xAB).all(), "wrote past the workspace"
+
+
+# --- the GELU on its whole range ----------------------------------------------
+
+def _gelu_of(ops, z, m, ot):
+    """GELU of the f32 values z (a bias on sums of zero), through the kernel for m rows; one row of it."""
+    import torch
+
+    n, k = z.numel(), 1040
+    x = torch.zeros(m, k, dtype=torch.int8, device="cuda")
+    w = torch.zeros(n, k, dtype=torch.int8, device="cuda")
+    out = _run_linear(ops, x, w, k, ot, None, None, z, 1)
+    assert (out == out[:1]).all() or out.isnan().any()
+    return out[0]
+
+
+# rows of the three kernels, and of tiles of both widths
+@pytest.mark.parametrize("m", [1, 2, 5, 20, 100, 700])
+@pytest.mark.parametrize("ot", ["f32", "f16", "bf16"])
+def test_gelu_and_its_tail(ops, m, ot):
+    # f32: the fit is within 5.2e-8 |z|, the roundings of its sum and products and
+    # ex2 (2^-22 of the exponential, at most 1/2 of which is R's) within 2.4e-7 |z|;
+    # every one of them shrinks with the exponential, and below -4 the fit's clamp is
+    # within 4.6 % of the value: the tail is held to 5 % of it, from -4 up to 0.3 %.
+    # ex2 is 0 below f32's normal numbers.
+    import torch
+
+    z = torch.cat([torch.linspace(-14, 14, 60001), torch.linspace(-0.01, 0.01, 2001),
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e5, -1e5, 3e38, -3e38])]).cuda()
+    zd = z.double()
+    tail = 0.5 * torch.special.erfc(zd.abs() / 2**0.5) * zd.abs()  # what max(z, 0) is less by
+    want = zd.clamp(min=0) - tail
+    bound = torch.minimum(3e-7 * zd.abs(), torch.where(zd.abs() > 4, 0.05, 0.003) * tail) + 2.0**-126 * zd.abs()
+    bound = bound + 2.0**-24 * want.abs()
+    got = _gelu_of(ops, z, m, ot)
+    big = HALF_ULP[ot] * (want.abs() + bound) + TINY[ot]
+    keep = want.abs() < (60000 if ot == "f16" else 1e38)  # others leave the type
+    _within(got[keep], want[keep], (bound + big)[keep], "gelu")
+
+
+@pytest.mark.parametrize("m", [1, 20, 700])
+def test_gelu_of_what_is_not_finite(ops, m):
+    import torch
+
+    inf, nan = float("inf"), float("nan")
+    got = _gelu_of(ops, torch.tensor([inf, -inf, nan, 1.0], device="cuda"), m, "f32")
+    assert got[0] == inf and got[1] == 0 and got[2].isnan() and 0.841 < got[3] < 0.842
