@@ -65,12 +65,12 @@ DMX_DEVICE float max_nan(float a, float b) {
 // with R(0) = 1/2 and the coefficients rounded to f32 one after the other from
 // the highest, the rest fitted anew each time. So rounded, it is off by at most
 // 5.1e-8 there, and by 1.5e-3 of E. Below -4 n stays while the exponential goes
-// on with z: n R(n) is within 4.6 % of its limit -1 / sqrt(2 pi) already, so the
+// on with z: n R(n) is within 4.7 % of its limit -1 / sqrt(2 pi) already, so the
 // tail keeps that relative error down to where f32 ends, and nothing overflows.
-// With f32's roundings: 1.2e-7 |z|, as the form by erff (1.1e-7), whose tail is
-// lost at -5.5. -infinity gives 0, a NaN stays one. One special-function
-// operation and paired FMAs a value; each step for all the pairs before the
-// next, so that a coefficient is set up once.
+// Measured over [-14, 14]: at most 1.4e-7 |z| off, and 2.3 % of the value at
+// -5.5 (the form by erff: 1.1e-7 |z|, and 57 %). -infinity gives 0, a NaN stays
+// one. One special-function operation and paired FMAs a value; each step for
+// all the pairs before the next, so that a coefficient is set up once.
 template <int P>
 DMX_DEVICE void gelu_pairs(float2* z) {
   constexpr float kR[11] = {0.5f,           0.39893952f,    0.249949172f,    0.132658452f,
@@ -608,7 +608,9 @@ DMX_DEVICE void tile_values(uint32_t tmem_at, const float4* col, float row_scale
     v[i] = scaled2((int)r[2 * i], (int)r[2 * i + 1], row_scale, make_float2(q.x, q.y),
                    make_float2(q.z, q.w));
   }
-  if (GELU) {  // in halves: with all eight pairs at once registers spill
+  if (GELU) {
+    // in halves, for fewer registers at once (112896x512->2048, with a polynomial
+    // of degree 11: 224 us against 230)
     gelu_pairs<4>(v);
     gelu_pairs<4>(v + 4);
   }
