@@ -5,7 +5,8 @@
 //
 // Three kernels, all on the same operands (rows on 16-byte boundaries, the
 // bytes past column k of a row never used):
-//  * linear_gemv_kernel: up to 8 rows, dp4a on weights streamed once;
+//  * linear_gemv_kernel: up to 8 rows and not too many weights, dp4a on weights
+//    streamed once;
 //  * linear_few_kernel: up to 128 rows and long k, tcgen05 with the weights as
 //    the 128-row operand, k split over a thread-block cluster;
 //  * linear_tile_kernel: the rest, persistent tcgen05 tiles.
@@ -968,10 +969,14 @@ bool launch_tile(const LinearArgs& a, cudaStream_t s) {
 template <typename OT, bool GELU>
 bool launch_typed(const LinearArgs& a, cudaStream_t s) {
   // A few rows: dp4a on streamed weights until its multiplications outweigh a
-  // tensor core tile's start. us for 8 rows: 512->512 2.6 against 3.8,
-  // 4096->4096 9.8 against 7.0; for 4: 4096->4096 5.9 against 7.0, 8192->8192 19
-  // against 15.0; for one 4096->4096 3.6 against 8.2.
-  if (a.rows <= 8 && a.rows * a.n * a.k <= 1ll << 26) {
+  // tensor core tile's start. us for 8 rows: 512->512 2.3 against 3.8,
+  // 4096->4096 9.8 against 7.0; for 4: 4096->4096 5.5 against 7.0, 8192->8192 19
+  // against 15.0; for one 4096->4096 2.8 against 8.2. One row of more weights:
+  // where k is short for a tile (1024->131072 24.8 against 44.8, 2048->40000 17.8
+  // against 21.2; 3000->30000 21.0 against 17.3, 8192->28672 44.4 against 40.8) or
+  // the channels make too few clusters for the SMs (65536->2048 25.6 against 27.4,
+  // 128000->700 25.2 against 35.8; 65536->4096 52.7 against 45.6).
+  if (a.rows <= 8 && (a.rows * a.n * a.k <= 1ll << 26 || (a.rows == 1 && (a.k <= 2048 || a.n <= 2048)))) {
     if (a.rows == 1) launch_gemv<1, 4, OT, GELU>(a, s);
     else if (a.rows == 2) launch_gemv<2, 4, OT, GELU>(a, s);
     else if (a.rows <= 4) launch_gemv<4, 4, OT, GELU>(a, s);

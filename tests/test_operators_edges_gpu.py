@@ -197,3 +197,20 @@ def test_gelu_of_what_is_not_finite(ops, m):
     inf, nan = float("inf"), float("nan")
     got = _gelu_of(ops, torch.tensor([inf, -inf, nan, 1.0], device="cuda"), m, "f32")
     assert got[0] == inf and got[1] == 0 and got[2].isnan() and 0.841 < got[3] < 0.842
+
+
+# --- one row of many weights --------------------------------------------------
+
+# both sides of where weights are streamed, and where k or the channels are few
+@pytest.mark.parametrize("n,k", [(70000, 1024), (33001, 2048), (32900, 2049), (40000, 2050), (8191, 8193), (8200, 8192),
+                                 (2048, 40000), (2049, 40001), (700, 128000), (1, 131071)])
+@pytest.mark.parametrize("ot", ["f32", "bf16"])
+def test_quantized_linear_of_one_row_and_many_weights(ops, n, k, ot):
+    x, w, xs, ws, b = _linear_inputs(1, n, k, n + k)
+    xs = xs / k**0.5
+    got = _run_linear(ops, x, w, k, ot, xs, ws, b)
+    # columns in pieces: the product in 64 bits of all of them would be gigabytes
+    for at in range(0, n, 8192):
+        part = slice(at, min(at + 8192, n))
+        want, bound = _linear_want(_product(x, w[part], k), xs, ws[part], b[part], 0, None, ot)
+        _within(got[:, part], want, bound, "out")
