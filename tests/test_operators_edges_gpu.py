@@ -214,3 +214,19 @@ def test_quantized_linear_of_one_row_and_many_weights(ops, n, k, ot):
         part = slice(at, min(at + 8192, n))
         want, bound = _linear_want(_product(x, w[part], k), xs, ws[part], b[part], 0, None, ot)
         _within(got[:, part], want, bound, "out")
+
+
+# --- long rows off 16 bytes ---------------------------------------------------
+
+# one, two and three blocks to an SM, by shifted vectors and (a weight of a third
+# type) by elements; more rows than blocks, so that each takes several
+@pytest.mark.parametrize("rows,cols", [(3001, 1031), (2003, 2001), (1801, 3001), (1501, 4097), (1203, 5003), (1001, 5201),
+                                       (801, 8191), (701, 8195), (503, 12001), (401, 16383)])
+@pytest.mark.parametrize("xt,dyt,params", [("bf16", "bf16", "bf16"), ("f32", "bf16", "f32"), ("f16", "f32", "bf16")])
+def test_backward_of_many_rows_off_16_bytes(ops, rows, cols, xt, dyt, params):
+    dy, x, w, mean, rstd = _back_inputs(rows, cols, xt, dyt, rows + cols, params)
+    dx, dw, db = _run_back(ops, dy, x, w, mean, rstd, params=params)
+    dx64, dw64, db64, e_dx, e_w, e_b = _back64(dy, x, w, mean, rstd)
+    _within(dx, dx64, e_dx + HALF_ULP[xt] * (dx64.abs() + e_dx) + TINY[xt], "dx")
+    _within(dw, dw64, e_w, "dweight")
+    _within(db, db64, e_b, "dbias")
