@@ -214,7 +214,7 @@ dmx_status dmx_ops_check(dmx_ops* ops, void* stream) {
     throw Error(DMX_ERR_TIMEOUT,
                 std::string(code == kSelftestCode ? "the self-test kernel" : "dmx_quantized_linear") +
                     ": a bounded wait gave up (code " + std::to_string(code) +
-                    "); the outputs of dmx_quantized_linear since the last check are not valid");
+                    "); what dmx_quantized_linear wrote on any stream since the last check is not valid");
   });
 }
 

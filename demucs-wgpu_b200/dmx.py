@@ -526,7 +526,8 @@ class Ops:
     __del__ = close
 
     def check(self, stream: int = 0):
-        """Waits for ``stream``; raises DmxError code 4 if a wait in a kernel gave up."""
+        """Waits for ``stream``; raises DmxError code 4 if a wait in a kernel of this
+        context, on any stream, gave up since the last check."""
         _check(self._L.dmx_ops_check(self._h, stream))
 
     def selftest_wait_timeout(self, wait_ms: int = 200, stream: int = 0):

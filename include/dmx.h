@@ -442,7 +442,12 @@ typedef struct dmx_ops dmx_ops;
 dmx_status dmx_ops_create(int device, dmx_ops** out);
 void dmx_ops_destroy(dmx_ops* ops);
 /* Waits (bounded) until `stream` has drained; DMX_ERR_TIMEOUT if a wait inside
- * a kernel of this context gave up since the last check (the flag is cleared). */
+ * a kernel of this context gave up since the last check. The flag is the
+ * context's, not the stream's: the first check after the failure reports it,
+ * on whichever stream, and clears it, and what dmx_quantized_linear wrote since
+ * the check before is then not valid on any stream, calls that were enqueued
+ * and had not run yet included. Programs that check streams apart give each a
+ * context of its own. */
 dmx_status dmx_ops_check(dmx_ops* ops, void* stream);
 /* Self-test of that path, as dmx_selftest_wait_timeout: enqueues one warp that
  * waits on a device flag that nothing sets, gives up after `wait_ms` (1..5000)

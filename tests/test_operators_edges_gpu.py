@@ -47,6 +47,24 @@ def test_calls_behind_a_raised_flag_end_and_the_next_ones_are_right(ops, m, n, k
         ops.check()
 
 
+def test_a_failure_is_the_contexts_and_reported_once_on_any_stream():
+    import dmx
+    import torch
+
+    one, other = dmx.Ops(0), dmx.Ops(0)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    one.selftest_wait_timeout(20, a.cuda_stream)
+    a.synchronize()
+    other.check(a.cuda_stream)  # another context: not its failure
+    with pytest.raises(dmx.DmxError, match="on any stream since the last check"):
+        one.check(b.cuda_stream)
+    for stream in (0, a.cuda_stream, b.cuda_stream):
+        one.check(stream)
+        other.check(stream)
+    one.close()
+    other.close()
+
+
 def test_the_self_test_of_a_wait_refuses_other_limits(ops):
     import dmx
 
