@@ -5,8 +5,9 @@ other calls. The plain implementations and bounds are test_operators_gpu.py's.
 
 import pytest
 
-from test_operators_gpu import (HALF_ULP, TINY, _back64, _back_inputs, _linear_inputs, _linear_want, _padded, _product,
-                                _run_back, _run_linear, _within)
+from test_operators_gpu import (HALF_ULP, TINY, U, _back64, _back_inputs, _linear_inputs, _linear_want, _norm64,
+                                _norm_bounds, _norm_inputs, _padded, _product, _quantise_steps, _run_back, _run_linear,
+                                _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +249,140 @@ def test_backward_of_many_rows_off_16_bytes(ops, rows, cols, xt, dyt, params):
     _within(dx, dx64, e_dx + HALF_ULP[xt] * (dx64.abs() + e_dx) + TINY[xt], "dx")
     _within(dw, dw64, e_w, "dweight")
     _within(db, db64, e_b, "dbias")
+
+
+# --- operands of different alignment ------------------------------------------
+
+CODE = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _placed(values, skip, pad=0, fill=7.0):
+    """The rows (or vector) at `skip` elements past an allocation's start, `pad` elements apart; and what is around."""
+    import torch
+
+    rows = values if values.dim() == 2 else values[None]
+    ld = rows.shape[1] + pad
+    flat = torch.full((skip + rows.shape[0] * ld + 3,), fill, dtype=values.dtype, device="cuda")
+    view = flat[skip:skip + rows.shape[0] * ld].view(rows.shape[0], ld)[:, :rows.shape[1]]
+    view.copy_(rows)
+    around = torch.ones_like(flat, dtype=torch.bool)
+    around[skip:skip + rows.shape[0] * ld].view(rows.shape[0], ld)[:, :rows.shape[1]] = False
+    return view if values.dim() == 2 else view[0], lambda: (flat[around] == fill).all()
+
+
+# (x, y, weight, bias): where each begins and the rows' padding
+@pytest.mark.parametrize("skips,pads", [((0, 1, 0, 0), (0, 0)), ((1, 0, 0, 0), (0, 0)), ((0, 0, 1, 0), (0, 0)),
+                                        ((0, 0, 0, 1), (0, 0)), ((4, 4, 4, 4), (0, 4)), ((8, 4, 0, 0), (8, 12)),
+                                        ((3, 5, 1, 2), (1, 2)), ((0, 0, 0, 0), (8, 1))])
+@pytest.mark.parametrize("rows,cols", [(9, 64), (700, 512), (5000, 512), (6, 2048), (900, 4104), (3, 17000)])
+@pytest.mark.parametrize("xt,yt,params", [("f32", "f32", "f32"), ("f32", "bf16", "f32"), ("f16", "f16", "f16")])
+def test_layer_norm_of_operands_of_different_alignment(ops, skips, pads, rows, cols, xt, yt, params):
+    import torch
+
+    x, w, b = _norm_inputs(rows, cols, xt, rows + cols, params)
+    xv, _ = _placed(x, skips[0], pads[0])
+    like = torch.zeros(rows, cols, device="cuda", dtype=dict(f32=torch.float32, f16=torch.float16,
+                                                             bf16=torch.bfloat16)[yt])
+    yv, alone = _placed(like, skips[1], pads[1])
+    wv, bv = _placed(w, skips[2])[0], _placed(b, skips[3])[0]
+    torch.cuda.synchronize()
+    ops.layer_norm(xv.data_ptr(), CODE[xt], rows, cols, yv.data_ptr(), CODE[yt], weight=wv.data_ptr(),
+                   bias=bv.data_ptr(), param_type=CODE[params], x_ld=xv.stride(0), y_ld=yv.stride(0))
+    torch.cuda.synchronize()
+    h, want, m64, r64 = _norm64(x, w, b, 1e-5)
+    e = _norm_bounds(x, h, want, w, m64, r64)[2]
+    _within(yv, want, e + HALF_ULP[yt] * (want.abs() + e) + TINY[yt], "y")
+    assert alone(), "wrote past the rows"
+
+
+# (dy, x, dx, weight), their padding, and the workspace's start in bytes
+@pytest.mark.parametrize("skips,pads,room_at", [((1, 0, 0, 0), (0, 0, 0), 0), ((0, 1, 0, 0), (0, 0, 0), 16),
+                                                ((0, 0, 1, 0), (0, 0, 0), 0), ((0, 0, 0, 1), (0, 0, 0), 0),
+                                                ((4, 0, 4, 4), (0, 0, 4), 48), ((8, 8, 0, 0), (8, 0, 16), 16),
+                                                ((3, 1, 5, 2), (1, 2, 0), 16), ((0, 0, 0, 0), (0, 0, 0), 16)])
+@pytest.mark.parametrize("rows,cols", [(40, 64), (1500, 512), (900, 2048), (320, 8200), (7, 17000)])
+@pytest.mark.parametrize("xt,dyt,params", [("f32", "f32", "f32"), ("f32", "bf16", "f32"), ("f16", "f16", "f16")])
+def test_backward_of_operands_of_different_alignment(ops, skips, pads, room_at, rows, cols, xt, dyt, params):
+    import torch
+
+    dy, x, w, mean, rstd = _back_inputs(rows, cols, xt, dyt, rows + cols, params)
+    dyv, xv = _placed(dy, skips[0], pads[0])[0], _placed(x, skips[1], pads[1])[0]
+    dxv, alone = _placed(torch.zeros_like(x), skips[2], pads[2])
+    wv = _placed(w, skips[3])[0]
+    dw, db = torch.empty(2, cols, device="cuda")
+    size = ops.layer_norm_backward_workspace(rows, cols)
+    room = torch.full((room_at + size + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ops.layer_norm_backward(dyv.data_ptr(), CODE[dyt], xv.data_ptr(), CODE[xt], mean.data_ptr(), rstd.data_ptr(), rows,
+                            cols, room.data_ptr() + room_at, size, weight=wv.data_ptr(), param_type=CODE[params],
+                            dx=dxv.data_ptr(), dweight=dw.data_ptr(), dbias=db.data_ptr(), dy_ld=dyv.stride(0),
+                            x_ld=xv.stride(0), dx_ld=dxv.stride(0))
+    torch.cuda.synchronize()
+    dx64, dw64, db64, e_dx, e_w, e_b = _back64(dy, x, w, mean, rstd)
+    _within(dxv, dx64, e_dx + HALF_ULP[xt] * (dx64.abs() + e_dx) + TINY[xt], "dx")
+    _within(dw, dw64, e_w, "dweight")
+    _within(db, db64, e_b, "dbias")
+    assert alone(), "wrote past the rows"
+    assert (room[:room_at] == 0xAB).all() and (room[room_at + size:] == 0xAB).all(), "wrote past the workspace"
+
+
+# (x, q, col_scale) and the padding of x and q
+@pytest.mark.parametrize("skips,pads", [((0, 1, 0), (0, 0)), ((1, 0, 0), (0, 0)), ((0, 0, 1), (0, 0)), ((4, 8, 4), (4, 8)),
+                                        ((0, 16, 0), (8, 3)), ((3, 5, 2), (1, 7))])
+@pytest.mark.parametrize("rows,cols", [(9, 64), (5000, 512), (300, 2048), (40, 8200), (3, 17000)])
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+def test_quantise_operands_of_different_alignment(ops, skips, pads, rows, cols, xt):
+    import numpy as np
+    import torch
+
+    x, w, _ = _norm_inputs(rows, cols, xt, rows + cols, "f32")
+    xv, wv = _placed(x, skips[0], pads[0])[0], _placed(w, skips[2])[0]
+    qv, alone = _placed(torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), skips[1], pads[1], 7)
+    scale = torch.empty(rows, device="cuda")
+    torch.cuda.synchronize()
+    ops.quantize_rows(xv.data_ptr(), CODE[xt], rows, cols, qv.data_ptr(), scale.data_ptr(), col_scale=wv.data_ptr(),
+                      x_ld=xv.stride(0), q_ld=qv.stride(0))
+    torch.cuda.synchronize()
+    want_q, want_scale = _quantise_steps((x.float() * w).cpu().numpy())
+    assert np.array_equal(scale.cpu().numpy(), want_scale) and np.array_equal(qv.cpu().numpy(), want_q)
+    assert alone(), "wrote past the rows"
+    # and with the norm before it, the same parameters as weight and bias
+    mean, rstd = torch.empty(2, rows, device="cuda")
+    ops.layer_norm_quantize(xv.data_ptr(), CODE[xt], rows, cols, qv.data_ptr(), scale.data_ptr(), weight=wv.data_ptr(),
+                            bias=wv.data_ptr(), x_ld=xv.stride(0), q_ld=qv.stride(0), mean=mean.data_ptr(),
+                            rstd=rstd.data_ptr())
+    torch.cuda.synchronize()
+    h, y, m64, r64 = _norm64(x, w, w, 1e-5)
+    e_mean, e_rstd, e_y = _norm_bounds(x, h, y, w, m64, r64)
+    _within(mean[:, None], m64, e_mean, "mean")
+    _within(rstd[:, None], r64, e_rstd, "rstd")
+    s = scale.double()[:, None]
+    off = (qv.double() - y / s).abs()
+    assert (off <= 0.5 + (e_y + 4 * U * y.abs()) / s + 1e-5).all(), off.max().item()
+    assert alone(), "wrote past the rows"
+
+
+# (out, residual, scales and bias) and the padding of out and residual
+@pytest.mark.parametrize("skips,pads", [((0, 1, 0), (0, 0)), ((1, 0, 0), (0, 0)), ((0, 0, 1), (0, 0)), ((4, 8, 3), (4, 8)),
+                                        ((8, 4, 0), (8, 4)), ((3, 5, 2), (1, 7))])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 512), (6, 136, 512), (20, 256, 2048), (100, 520, 2048), (300, 512, 256),
+                                   (3000, 1032, 512)])
+@pytest.mark.parametrize("ot", ["f32", "f16"])
+def test_linear_operands_of_different_alignment(ops, skips, pads, m, n, k, ot):
+    import torch
+
+    x, w, xs, ws, b = _linear_inputs(m, n, k, m + n + k)
+    xs = xs / k**0.5
+    dtype = dict(f32=torch.float32, f16=torch.float16)[ot]
+    r = torch.randn(m, n, device="cuda").to(dtype)
+    ov, alone = _placed(torch.zeros_like(r), skips[0], pads[0])
+    rv = _placed(r, skips[1], pads[1])[0]
+    xsv, wsv, bv = (_placed(t, skips[2])[0] for t in (xs, ws, b))
+    torch.cuda.synchronize()
+    ops.quantized_linear(x.data_ptr(), w.data_ptr(), ov.data_ptr(), CODE[ot], m, n, k, x_scale=xsv.data_ptr(),
+                         w_scale=wsv.data_ptr(), bias=bv.data_ptr(), residual=rv.data_ptr(), x_ld=x.stride(0),
+                         w_ld=w.stride(0), residual_ld=rv.stride(0), out_ld=ov.stride(0))
+    torch.cuda.synchronize()
+    want, bound = _linear_want(_product(x, w, k), xs, ws, b, 0, r, ot)
+    _within(ov, want, bound, "out")
+    assert alone(), "wrote past the rows"
