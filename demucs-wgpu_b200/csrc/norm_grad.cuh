@@ -16,7 +16,8 @@
 // than that are swept twice, for dx and for the column sums, re-read from L2.
 // Measured: 112896 x 512 f32 with bf16 gradients 95 us (6070 GB/s), 28000 x 2048
 // bf16 82 us (4180), 4095 x 8195 bf16 66 us (3050: the block-wide reductions of
-// each row), 20000 x 5001 bf16 off 16 bytes 290 us (2070).
+// each row), 20000 x 5001 bf16 off 16 bytes 290 us (2070; 312 with
+// an f32 weight).
 #pragma once
 
 #include <algorithm>
@@ -494,10 +495,15 @@ void launch_norm_grad_vec(const NormGradArgs& a, int parts, bool wide, cudaStrea
     const int ahead = VEC ? std::min(4, (most - own) / stage) : 0;
     const dim3 block(threads, groups);
     const size_t smem = (size_t)threads * groups * (own + ahead * stage);
-    // two rows at a time where registers and copies allow it
+    // Built for the registers that a block's threads leave each of them. Up to 512
+    // threads (8192 columns) 128, two rows at a time (28000 x 2048 bf16: 82 us, one
+    // at a time 94; 7000 x 8192 f32 181 and 195). Up to 640 (10240 columns) 96, one
+    // row at a time; with the 64 of 1024 threads values spill: 4000 x 9216 bf16 65
+    // us against 114, 3000 x 10240 f32 with bf16 gradients 87 against 148. Longer
+    // rows have the 64 all the same (3000 x 12288 bf16 92 us).
     if constexpr (!VEC)
       launch_norm_grad_block<XT, DT, PT, BY_ELEMENT, 1024, 1>(a, parts, block, smem, wide, ahead, s);
-    else if (ahead < 1)  // no room to copy ahead: rows go by elements
+    else if (ahead < 1)  // no room to copy ahead: rows go by elements (2500 x 16384 f32: 199 us)
       launch_norm_grad_block<XT, DT, Any, BY_ELEMENT, 1024, 1>(a, parts, block, smem, wide, ahead, s);
     else if (threads * groups <= 512 && ahead >= 2)
       launch_norm_grad_block<XT, DT, PT, BY_VECTOR, 512, 2>(a, parts, block, smem, wide, ahead, s);

@@ -10,10 +10,10 @@
 //  * linear_few_kernel: up to 128 rows and long k, tcgen05 with the weights as
 //    the 128-row operand, k split over a thread-block cluster;
 //  * linear_tile_kernel: the rest, persistent tcgen05 tiles.
-// The first two are bound by the weights' bytes (1 x 8192 -> 8192: 13.6 us, 4.9
-// TB/s), the last by the tensor core where k is long (8192^3: 358 us, 3.07
+// The first two are bound by the weights' bytes (1 x 8192 -> 8192: 14.3 us, 4.7
+// TB/s), the last by the tensor core where k is long (8192^3: 356 us, 3.09
 // POP/s) and by its epilogue or HBM where it is short (112896 x 512 -> 2048 to
-// bf16: 150 us; with GELU 214).
+// bf16: 150 us; with GELU 212).
 #include <algorithm>
 
 #include "ops.h"
@@ -970,7 +970,7 @@ template <typename OT, bool GELU>
 bool launch_typed(const LinearArgs& a, cudaStream_t s) {
   // A few rows: dp4a on streamed weights until its multiplications outweigh a
   // tensor core tile's start. us for 8 rows: 512->512 2.3 against 3.8,
-  // 4096->4096 9.8 against 7.0; for 4: 4096->4096 5.5 against 7.0, 8192->8192 19
+  // 4096->4096 8.6 against 6.9; for 4: 4096->4096 5.5 against 7.0, 8192->8192 21.3
   // against 15.0; for one 4096->4096 2.8 against 8.2. One row of more weights:
   // where k is short for a tile (1024->131072 24.8 against 44.8, 2048->40000 17.8
   // against 21.2; 3000->30000 21.0 against 17.3, 8192->28672 44.4 against 40.8) or
